@@ -463,6 +463,57 @@ int b200q_nvfp4_gemm(const uint8_t* a, const uint8_t* b, const uint8_t* sfa, con
 int b200q_nvfp4_swizzle_scales(const uint8_t* scales, uint8_t* swizzled, int64_t rows, int64_t cols,
                                void* stream);
 
+/* ---------------------------------------------------------------- paged NVFP4 KV cache ------ */
+
+/* One step of a paged KV cache, from lengths on the device.  Request b holds lens[b] tokens and adds
+ * new_lens[b]; table [requests, width] (rows table_stride apart) holds its page ids, of which the first
+ * ceil(lens[b] / page) are read.  free_pages[*taken ...] are the ids that may be handed out.  Written:
+ *   table[b, ceil(lens[b]/page) .. ceil((lens[b]+new_lens[b])/page))   the pages taken, in request order
+ *   cu_new[b] = rows of the requests before b (requests + 1 entries)
+ *   slots[t], positions[t] of token row t = cu_new[b] + i: the token's position lens[b] + i and
+ *     table[b, position / page] * page + position % page; -1 and 0 for rows behind the last request
+ *   lens_out[b] = lens[b] + new_lens[b], *taken_out = *taken + pages taken
+ * A request that does not fit is refused: its length stays, its rows get slot -1, and *status is the OR of
+ * 1 (free list exhausted: this request and the later ones that need a page), 2 (wider than its table row),
+ * 4 (negative or too large a length), 8 (more new tokens than rows).  lens_out and taken_out must not
+ * overlap the inputs; the call may be repeated on the same inputs.  At most 8192 requests.  Pointers need
+ * their element's alignment only. */
+int b200q_kv_step(const int* lens, const int* new_lens, const int* free_pages, int nfree, const int* taken, int* table,
+                  int64_t table_stride, int width, int requests, int page, int tokens, int64_t* slots, int* positions,
+                  int* cu_new, int* lens_out, int* taken_out, int* status, void* stream);
+
+/* New keys and values quantised to NVFP4 and written at their slots.  k, v: [tokens, heads, dim] of type T with
+ * the given strides in elements (last dimension contiguous; pointers and strides multiples of 32 bytes), dim a
+ * multiple of 16.  Codes [pages, heads, page, dim/2] (even element in the low nibble) and E4M3 block scales
+ * [pages, heads, page, dim/16]; k_scale2, v_scale2 device fp32 scalars (amax / 2688).  The arithmetic of
+ * b200q_nvfp4_quantize with B200Q_NVFP4_SATURATE_SCALES.  A slot outside [0, pages * page) is not written;
+ * slots must be distinct (two rows of one slot leave a mix of both).  k_values, v_values
+ * [tokens, heads, dim] of type T, each may be NULL: the values the cache now stands for. */
+int b200q_nvfp4_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_token_stride, int64_t v_head_stride, int dtype, const int64_t* slots, int tokens,
+                          int heads, int dim, const float* k_scale2, const float* v_scale2, uint8_t* k_codes,
+                          uint8_t* k_scales, uint8_t* v_codes, uint8_t* v_scales, int pages, int page, void* k_values,
+                          void* v_values, void* stream);
+
+/* Attention of a step's tokens over the cache: out[t, h*group + g] = softmax(scale * q . K^T) V over the tokens
+ * that query t sees.  Request b owns token rows cu_q[b] .. cu_q[b+1] of q (cu_q NULL: row b alone, tokens ==
+ * requests); they are the last of its lens[b] cached tokens, and query i of n sees positions
+ * 0 .. lens[b] - n + i.  A row that sees nothing (an empty request) gives zeros and lse -inf.
+ * q: [tokens, heads * group, dim] of type T (B200Q_F16 or B200Q_BF16) with the given strides (elements,
+ * multiples of 8; last dimension contiguous); out contiguous of type T; lse [tokens, heads * group] fp32 (natural
+ * logarithm) or NULL.  dim 64, 128 or 256; page a multiple of 16; table rows as in b200q_kv_step (an id outside
+ * [0, pages) hides its tokens; lens beyond width * page are cut).  Rows of q at and behind cu_q[requests] are not
+ * computed: their output is left as it is, or zeroed (lse -inf) where zero_tail != 0.
+ * workspace: b200q_nvfp4_kv_attention_workspace(...) bytes, this call's alone until it has run; *status_io as in
+ * b200q_fp8_gemm.  Lengths are read on the device only: the call can be captured and replayed with others. */
+int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
+                             const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                             const uint8_t* v_scales, const float* k_scale2, const float* v_scale2, const int* table,
+                             int64_t table_stride, int width, const int* lens, const int* cu_q, int requests, int tokens,
+                             int heads, int group, int dim, int pages, int page, float scale, void* out, float* lse,
+                             int zero_tail, void* workspace, int64_t workspace_bytes, uint32_t* status_io, void* stream);
+int64_t b200q_nvfp4_kv_attention_workspace(int tokens, int requests, int heads, int group, int dim);
+
 /* ---------------------------------------------------------------- export packers ------------ */
 
 /* INT4 weights in the checkpoint layout: q = clamp(round_half_even(w / scale[r, c/block]), -8, 7)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -885,3 +886,206 @@ def nvfp4_gemm(a4: torch.Tensor, sfa: torch.Tensor, b4: torch.Tensor, sfb: torch
              bias.data_ptr() if bias is not None else None, out.data_ptr(), m, n, k, _DT[out_dtype],
              qgemm_status(a4.device).data_ptr(), _stream(a4))
     return out
+
+
+# --------------------------------------------------------------------------- paged NVFP4 KV cache --
+
+class KvStep(NamedTuple):
+    """What ``kv_step`` returns (all on the device): ``slots`` int64 and ``positions`` int32 per token row,
+    ``cu_new`` int32 [requests + 1] first row of each request, ``lens`` int32 the lengths after the step,
+    ``taken`` int32 [1] free pages handed out so far, ``status`` int32 [1] (0 = every request was served)."""
+
+    slots: torch.Tensor
+    positions: torch.Tensor
+    cu_new: torch.Tensor
+    lens: torch.Tensor
+    taken: torch.Tensor
+    status: torch.Tensor
+
+
+def _int32_vector(t: torch.Tensor, what: str, device=None) -> torch.Tensor:
+    _cuda(t, what)
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"b200q: {what} must be a contiguous one-dimensional int32 tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"b200q: {what} is on {t.device}, expected {device}")
+    return t
+
+
+def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
+            block_table: torch.Tensor, page_size: int, tokens: int) -> KvStep:
+    """Page table entries, slots and positions of one step, built on the device in one launch.
+
+    Request b holds ``lens[b]`` tokens and adds ``new_lens[b]`` (int32); ``block_table`` [requests, width]
+    int32 holds its page ids and receives the new ones IN PLACE, taken in request order from
+    ``free_pages[taken:]``.  ``tokens`` is the number of token rows of the step's tensors; rows behind the
+    last request get slot -1.  A request that does not fit (free list, table row, rows, a negative length)
+    is refused: it keeps its length, its rows get slot -1, and ``status`` is not zero (bits 1, 2, 8, 4).
+    The inputs other than the table stay as they are; repeating the call gives the same result."""
+    lens = _int32_vector(lens, "lens")
+    dev, b = lens.device, lens.numel()
+    new_lens = _int32_vector(new_lens, "new_lens", dev)
+    free_pages = _int32_vector(free_pages, "free_pages", dev)
+    taken = _int32_vector(taken, "taken", dev)
+    _cuda(block_table, "block_table")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("b200q: block_table must be a two-dimensional int32 tensor with contiguous rows")
+    if new_lens.numel() != b or block_table.shape[0] != b or taken.numel() != 1:
+        raise ValueError("b200q: lens, new_lens and block_table must have one entry per request, taken exactly one")
+    if b == 0 or page_size <= 0 or tokens < 0:
+        raise ValueError("b200q: kv_step needs at least one request, a positive page size and tokens >= 0")
+    if b > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("b200q: the rows of block_table overlap")
+    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    ints = torch.empty(2 * b + 3 + tokens, dtype=torch.int32, device=dev)
+    cu, lens_out, taken_out, status, positions = ints.split((b + 1, b, 1, 1, tokens))
+    at = ints.data_ptr()
+    with _on(dev):
+        call("b200q_kv_step", lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(),
+             taken.data_ptr(), block_table.data_ptr(), block_table.stride(0) if b > 1 else block_table.shape[1],
+             block_table.shape[1], b, page_size, tokens, slots.data_ptr(), at + 4 * (2 * b + 3), at, at + 4 * (b + 1),
+             at + 4 * (2 * b + 1), at + 4 * (2 * b + 2), _stream(lens))
+    return KvStep(slots, positions, cu, lens_out, taken_out, status)
+
+
+def _kv_pages(cache, what: str, device=None):
+    """(codes, scales) of one side of a cache, checked -> (codes, scales, pages, heads, page size, dim)."""
+    codes, scales = cache
+    _cuda(codes, what), _cuda(scales, what)
+    if codes.dim() != 4 or scales.dim() != 4 or codes.dtype != torch.uint8 or scales.element_size() != 1:
+        raise ValueError(f"b200q: {what} must be (codes uint8 [pages, heads, page, dim/2], scales float8_e4m3fn "
+                         "[pages, heads, page, dim/16])")
+    pages, heads, page, half = codes.shape
+    if scales.shape != (pages, heads, page, half // 8) or half % 8:
+        raise ValueError(f"b200q: the scales of {what} do not match its codes")
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f"b200q: {what} must be contiguous")
+    if codes.device != scales.device or (device is not None and codes.device != device):
+        raise ValueError(f"b200q: {what} is on another device")
+    return codes, scales, pages, heads, page, 2 * half
+
+
+def _kv_scale2(s: torch.Tensor, device) -> torch.Tensor:
+    if s.dtype == torch.float32 and s.device == device and s.numel() == 1:
+        return s
+    s = _amax_f32(s, device)
+    if s.numel() != 1:
+        raise ValueError("b200q: k_scale2 and v_scale2 are one number each")
+    return s
+
+
+def _kv_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [tokens, heads, dim] as the append reads it: last dimension contiguous, 32-byte aligned rows (a view of a
+    fused projection's output usually is; anything else is copied)."""
+    es = x.element_size()
+    if (x.stride(2) == 1 and x.stride(0) >= 0 and x.stride(1) >= 0
+            and not ((x.data_ptr() | x.stride(0) * es | x.stride(1) * es) & 31)):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def nvfp4_kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor,
+                    v_scale2: torch.Tensor, return_values: bool = False):
+    """Quantise ``k`` and ``v`` [tokens, heads, dim] to NVFP4 and write them at ``slots`` (int64 [tokens], distinct;
+    a negative slot or one beyond the cache is skipped).  ``k_cache``, ``v_cache``: (codes uint8
+    [pages, heads, page, dim/2], scales float8_e4m3fn [pages, heads, page, dim/16]), updated in place; ``k_scale2``,
+    ``v_scale2``: fp32 amax / 2688 of the calibrated amax (a block beyond it saturates).  With ``return_values`` the
+    values that the cache now stands for come back as (k, v) in the inputs' dtype, padded rows included: what the
+    prompt's own attention reads to agree with later steps."""
+    _cuda(k, "k"), _cuda(v, "v"), _cuda(slots, "slots")
+    dev = k.device
+    kc, ks, pages, heads, page, dim = _kv_pages(k_cache, "k_cache", dev)
+    vc, vs, *vshape = _kv_pages(v_cache, "v_cache", dev)
+    if vshape != [pages, heads, page, dim]:
+        raise ValueError("b200q: k_cache and v_cache differ in shape")
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or v.device != dev or k.shape[1:] != (heads, dim):
+        raise ValueError(f"b200q: k and v must be [tokens, {heads}, {dim}] tensors of one dtype and device")
+    if slots.dtype != torch.int64 or slots.shape != k.shape[:1] or not slots.is_contiguous() or slots.device != dev:
+        raise ValueError("b200q: slots must be a contiguous int64 tensor with one entry per token")
+    dt = dtype_code(k)
+    tokens = k.shape[0]
+    kv = vv = None
+    if return_values:
+        kv, vv = (torch.empty((tokens, heads, dim), dtype=k.dtype, device=dev) for _ in range(2))
+    if tokens:
+        k, v = _kv_rows(k), _kv_rows(v)
+        k2, v2 = _kv_scale2(k_scale2, dev), _kv_scale2(v_scale2, dev)
+        ktok, khead, _ = k.stride()
+        vtok, vhead, _ = v.stride()
+        with _on(dev):
+            call("b200q_nvfp4_kv_append", k.data_ptr(), ktok, khead, v.data_ptr(), vtok, vhead, dt, slots.data_ptr(), tokens,
+                 heads, dim, k2.data_ptr(), v2.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+                 pages, page, kv.data_ptr() if return_values else None, vv.data_ptr() if return_values else None,
+                 _stream(k))
+    return (kv, vv) if return_values else None
+
+
+_KV_DIMS = (64, 128, 256)
+
+
+def nvfp4_kv_attention_supported(q: torch.Tensor, heads: int, page: int) -> bool:
+    """Whether ``nvfp4_kv_attention`` covers q [tokens, query heads, dim] over a cache of ``heads`` kv heads."""
+    return (q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and q.shape[2] in _KV_DIMS
+            and heads > 0 and q.shape[1] % heads == 0 and page > 0 and page % 16 == 0)
+
+
+def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor, v_scale2: torch.Tensor,
+                       block_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor | None = None,
+                       scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Causal attention of a step's tokens over the paged NVFP4 cache -> ``out`` [tokens, query heads, dim] in q's
+    dtype, with ``return_lse`` also the fp32 log-sum-exp [tokens, query heads].
+
+    ``q`` [tokens, query heads, dim] float16 / bfloat16, dim 64, 128 or 256, query heads a multiple of the cache's;
+    ``lens`` int32 [requests]: tokens of each request in the cache, the step's own included; ``block_table`` int32
+    [requests, width].  Without ``cu_q`` every request has one query; with it (int32 [requests + 1]) request b owns
+    rows cu_q[b] : cu_q[b + 1], its last tokens, each seeing everything up to itself.  Rows that see nothing are
+    zero (lse -inf), and so are rows behind the last request unless ``out`` is given, which keeps them.  ``scale``
+    defaults to dim ** -0.5.  Lengths are read on the device: a captured call serves later lengths too."""
+    _cuda(q, "q")
+    dev = q.device
+    kc, ks, pages, heads, page, dim = _kv_pages(k_cache, "k_cache", dev)
+    vc, vs, *vshape = _kv_pages(v_cache, "v_cache", dev)
+    if vshape != [pages, heads, page, dim]:
+        raise ValueError("b200q: k_cache and v_cache differ in shape")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"b200q: nvfp4_kv_attention takes float16 or bfloat16 queries, got {q.dtype}")
+    if not nvfp4_kv_attention_supported(q, heads, page) or q.shape[2] != dim or q.shape[1] == 0:
+        raise ValueError(f"b200q: nvfp4_kv_attention covers q [tokens, n * {heads}, {dim}] with dim 64, 128 or 256 and "
+                         f"page sizes that are multiples of 16; got q {tuple(q.shape)}, page {page}")
+    lens = _int32_vector(lens, "lens", dev)
+    _cuda(block_table, "block_table")
+    b, tokens, qheads = lens.numel(), q.shape[0], q.shape[1]
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev
+            or block_table.shape[0] != b or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError("b200q: block_table must be int32 [requests, width] with contiguous rows")
+    if cu_q is None:
+        if tokens != b:
+            raise ValueError("b200q: without cu_q there is one query per request")
+    else:
+        cu_q = _int32_vector(cu_q, "cu_q", dev)
+        if cu_q.numel() != b + 1:
+            raise ValueError("b200q: cu_q must have requests + 1 entries")
+    zero_tail = out is None
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("b200q: out must be a contiguous, 16-byte aligned tensor like q")
+    lse = torch.empty((tokens, qheads), dtype=torch.float32, device=dev) if return_lse else None
+    if b == 0 or tokens == 0:
+        out.zero_() if zero_tail else None
+        return (out, lse.fill_(float("-inf"))) if return_lse else out
+    if q.stride(2) != 1 or (q.data_ptr() | 2 * q.stride(0) | 2 * q.stride(1)) & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+    k2, v2 = _kv_scale2(k_scale2, dev), _kv_scale2(v_scale2, dev)
+    group = qheads // heads
+    with _on(dev):
+        need = call("b200q_nvfp4_kv_attention_workspace", tokens, b, heads, group, dim)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)   # this call's own: the allocator orders its reuse
+        call("b200q_nvfp4_kv_attention", q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q), kc.data_ptr(), ks.data_ptr(),
+             vc.data_ptr(), vs.data_ptr(), k2.data_ptr(), v2.data_ptr(), block_table.data_ptr(),
+             block_table.stride(0) if b > 1 else block_table.shape[1], block_table.shape[1], lens.data_ptr(),
+             cu_q.data_ptr() if cu_q is not None else None, b, tokens, heads, group, dim, pages, page,
+             dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr() if return_lse else None,
+             int(zero_tail), ws.data_ptr(), need, qgemm_status(dev).data_ptr(), _stream(q))
+    return (out, lse) if return_lse else out
