@@ -463,6 +463,23 @@ int b200q_nvfp4_gemm(const uint8_t* a, const uint8_t* b, const uint8_t* sfa, con
 int b200q_nvfp4_swizzle_scales(const uint8_t* scales, uint8_t* swizzled, int64_t rows, int64_t cols,
                                void* stream);
 
+/* ---------------------------------------------------------------- few rows, 4-bit weights ---- */
+
+/* out[m, n] = T(sum_k x[m, k] W[n, k] + bias[n]) for a few rows of x and a packed weight that is read once and
+ * never dequantised to memory; fp32 sums, one rounding.
+ *   b200q_int4_linear    W = (code - 8) / scales[n, k/block], codes as b200q_int4_quantize packs them (even element
+ *                        in the high nibble), scales of type T; block 32, 64 or a multiple of 128 that divides k
+ *   b200q_nvfp4_linear   W = e2m1 * scales[n, k/16] * (*scale2), codes as b200q_nvfp4_quantize packs them
+ * T is B200Q_F16 or B200Q_BF16.  x rows x_stride and out rows out_stride elements apart; x, its stride (in bytes) and
+ * codes 16-byte aligned, k a multiple of 32; bias [n] of type T or NULL.  At most 32 rows, and x has to fit on chip:
+ * rows up to b200q_w4_linear_max_rows(k) (0: none), more give B200Q_ERR_CAPACITY. */
+int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const void* scales, int block,
+                      const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, void* stream);
+int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales,
+                       const float* scale2, const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k,
+                       void* stream);
+int b200q_w4_linear_max_rows(int64_t k);
+
 /* ---------------------------------------------------------------- paged NVFP4 KV cache ------ */
 
 /* One step of a paged KV cache, from lengths on the device.  Request b holds lens[b] tokens and adds

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -971,7 +972,7 @@ def _kv_scale2(s: torch.Tensor, device) -> torch.Tensor:
         return s
     s = _amax_f32(s, device)
     if s.numel() != 1:
-        raise ValueError("b200q: k_scale2 and v_scale2 are one number each")
+        raise ValueError("b200q: a per-tensor scale is one number")
     return s
 
 
@@ -1089,3 +1090,76 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
              dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr() if return_lse else None,
              int(zero_tail), ws.data_ptr(), need, qgemm_status(dev).data_ptr(), _stream(q))
     return (out, lse) if return_lse else out
+
+
+# --------------------------------------------------------------------------- few rows, 4-bit weights --
+
+def w4_linear_supported(x: torch.Tensor, k: int, block: int) -> bool:
+    """Whether ``int4_linear`` (``block`` its group) / ``nvfp4_linear`` (block 16) cover x [..., k]."""
+    return (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1 and x.shape[-1] == k
+            and k % 32 == 0 and block > 0 and k % block == 0 and (block in (16, 32, 64) or block % 128 == 0)
+            and _w4_max_rows(k) > 0)
+
+
+@functools.lru_cache(maxsize=None)
+def _w4_max_rows(k: int) -> int:
+    return call("b200q_w4_linear_max_rows", k)
+
+
+def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, extra, bias):
+    _cuda(x, "x"), _cuda(packed, "packed"), _cuda(scales, "scales")
+    dev = x.device
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"b200q: products with 4-bit weights take float16 or bfloat16 rows, got {x.dtype}")
+    if packed.dim() != 2 or packed.element_size() != 1:
+        raise ValueError("b200q: packed must be [n, k/2] bytes")
+    n, k = packed.shape[0], 2 * packed.shape[1]
+    if n == 0 or not w4_linear_supported(x, k, block):
+        raise ValueError(f"b200q: no 4-bit product for x {tuple(x.shape)}, weight [{n}, {k}], block {block}")
+    if scales.numel() != n * (k // block):
+        raise ValueError(f"b200q: expected {n * (k // block)} scales, got {scales.numel()}")
+    for t in (packed, scales) if bias is None else (packed, scales, bias):
+        if t.device != dev:
+            raise ValueError("b200q: x, weight and bias must be on one device")
+    if bias is not None:
+        if bias.numel() != n:
+            raise ValueError(f"b200q: bias must have {n} elements")
+        bias = bias.detach().to(x.dtype).contiguous()
+    packed, scales = _prep(packed), scales.contiguous()
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    if x2.stride(1) != 1 or (x2.data_ptr() | 2 * x2.stride(0)) & 15:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    m = x2.shape[0]
+    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
+    most = _w4_max_rows(k)
+    with _on(dev):
+        for r in range(0, m, most):
+            call(name, x2.data_ptr() + 2 * r * x2.stride(0), x2.stride(0), _DT[x.dtype], packed.data_ptr(), scales.data_ptr(),
+                 extra, bias.data_ptr() if bias is not None else None, out.data_ptr() + 2 * r * n, n, min(most, m - r), n, k,
+                 _stream(x))
+    return out
+
+
+def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, bias: torch.Tensor | None = None):
+    """x [..., k] times an INT4 weight -> [..., n] in x's dtype: W = (code - 8) / scale, ``packed`` uint8 [n, k/2] (even
+    element in the high nibble) and ``scales`` [n * k/block, 1] in x's dtype as ``int4_quantize`` gives them for a
+    weight whose rows are whole blocks.  float16 / bfloat16; block 32, 64 or a multiple of 128.  The weight is read
+    once for every 32 rows (fewer where k is very long), without being dequantised to memory: for decoding batches; a
+    long prompt is faster through ``int4_dequantize`` and a GEMM."""
+    if scales.dtype != x.dtype:
+        raise TypeError(f"b200q: int4_linear takes scales of x's dtype {x.dtype}, got {scales.dtype}")
+    if block == 16:
+        raise ValueError("b200q: int4_linear covers groups of 32, 64 and multiples of 128")
+    return _w4_linear("b200q_int4_linear", x, packed, scales, block, block, bias)
+
+
+def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, scale2: torch.Tensor,
+                 bias: torch.Tensor | None = None):
+    """x [..., k] times an NVFP4 weight, x left in 16 bits -> [..., n] in x's dtype: W = e2m1 * scale * scale2 with
+    ``packed`` uint8 [n, k/2], ``scales`` float8_e4m3fn [n, k/16] and ``scale2`` fp32 as ``nvfp4_quantize`` gives them.
+    Like ``int4_linear`` in everything else."""
+    if scales.element_size() != 1:
+        raise TypeError("b200q: nvfp4_linear takes float8_e4m3fn scales")
+    _cuda(x, "x")
+    s2 = _kv_scale2(scale2, x.device)
+    return _w4_linear("b200q_nvfp4_linear", x, packed, scales, 16, s2.data_ptr(), bias)

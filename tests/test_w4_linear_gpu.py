@@ -1,0 +1,207 @@
+"""Products of a few rows with 4-bit weights (INT4 with group scales, NVFP4) against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+E2M1 = [0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6]
+
+
+def _int4(n, k, block, dtype, seed):
+    from b200q import ops
+
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    w = (torch.randn(n, k, generator=g, device=DEV) * torch.logspace(-3, 0, n, device=DEV).unsqueeze(1)).to(dtype)
+    packed, scales = ops.int4_quantize(w.reshape(-1), block)
+    packed = packed.reshape(n, k // 2)
+    c = torch.stack((packed >> 4, packed & 15), -1).reshape(n, k // block, block).double()
+    return packed, scales, ((c - 8) / scales.reshape(n, -1, 1).double()).reshape(n, k)
+
+
+def _nvfp4(n, k, dtype, seed):
+    from b200q import ops
+
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    w = (torch.randn(n, k, generator=g, device=DEV) * torch.logspace(-3, 0, n, device=DEV).unsqueeze(1)).to(dtype)
+    packed, scales, s2 = ops.nvfp4_quantize(w)
+    lut = torch.tensor(E2M1, dtype=torch.float64, device=DEV)
+    v = lut[torch.stack((packed & 15, packed >> 4), -1).reshape(n, k).long()]
+    return packed, scales, s2, (v.reshape(n, -1, 16) * scales.float().double().unsqueeze(-1)).reshape(n, k) * s2.double()
+
+
+def _close(out, x, w, bias=None):
+    """Half a step of the output's type, the fp32 sums (k + 8 operations, each off by at most 2^-23 of the sum of
+    magnitudes; the tensor core may truncate where it adds), the group's reciprocal and its product (2^-22), and x's
+    smallest elements in fp16 (2^-38 of the row's largest)."""
+    ref = x.double() @ w.t()
+    size = x.double().abs() @ w.abs().t()
+    if bias is not None:
+        ref = ref + bias.double()
+        size = size + bias.double().abs()
+    info = torch.finfo(out.dtype)
+    tol = (info.eps / 2 * ref.abs().clamp(min=info.tiny) + size * ((x.shape[-1] + 8) * 2.0 ** -23 + 2.0 ** -21)
+           + 2.0 ** -38 * x.double().abs().amax(-1, keepdim=True) * w.abs().sum(1)) * 1.01
+    assert out.shape == ref.shape
+    assert float(((out.double() - ref).abs() - tol).max()) <= 0
+
+
+def _x(m, k, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(100 + seed)
+    x = torch.randn(m, k, generator=g, device=DEV)
+    x[:, ::53] *= 30
+    return x.to(dtype)
+
+
+SIZES = [(1, 32), (16, 128), (17, 160), (33, 2080), (100, 4096), (4097, 256), (48, 14336), (64, 8320)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 16, 27, 32])
+@pytest.mark.parametrize("n,k", SIZES)
+def test_nvfp4_linear(dtype, m, n, k):
+    from b200q import ops
+
+    packed, scales, s2, w = _nvfp4(n, k, dtype, seed=n + m)
+    x = _x(m, k, dtype, m)
+    _close(ops.nvfp4_linear(x, packed, scales, s2), x, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 2, 7, 13, 30])
+@pytest.mark.parametrize("n,k,block", [(1, 32, 32), (20, 96, 32), (15, 64, 64), (77, 2112, 64), (16, 128, 128), (130, 2688, 128),
+                                       (4099, 384, 128), (40, 14336, 128), (33, 1024, 256), (7, 8192, 1024), (24, 28672, 32)])
+def test_int4_linear(dtype, m, n, k, block):
+    from b200q import ops
+
+    packed, scales, w = _int4(n, k, block, dtype, seed=n + m)
+    x = _x(m, k, dtype, m)
+    _close(ops.int4_linear(x, packed, scales, block), x, w)
+
+
+@pytest.mark.parametrize("m,k", [(33, 512), (70, 128), (40, 28672)])
+def test_more_rows_than_one_launch_takes(m, k):
+    from b200q import ops
+
+    packed, scales, s2, w = _nvfp4(50, k, torch.bfloat16, seed=1)
+    x = _x(m, k, torch.bfloat16)
+    _close(ops.nvfp4_linear(x, packed, scales, s2), x, w)
+
+
+def test_bias_shapes_and_strides():
+    from b200q import ops
+
+    n, k = 70, 512
+    packed, scales, s2, w = _nvfp4(n, k, torch.float16, seed=1)
+    bias = torch.randn(n, device=DEV)                     # cast to x's dtype
+    x = _x(6, k, torch.float16)
+    want = ops.nvfp4_linear(x, packed, scales, s2, bias)
+    _close(want, x, w, bias.half())
+    assert torch.equal(ops.nvfp4_linear(x.view(2, 3, k), packed, scales, s2, bias), want.view(2, 3, n))
+    assert torch.equal(ops.nvfp4_linear(x[0], packed, scales, s2, bias), want[0])
+    wide = torch.zeros(6, 2 * k, dtype=x.dtype, device=DEV)
+    wide[:, k:] = x
+    assert torch.equal(ops.nvfp4_linear(wide[:, k:], packed, scales, s2, bias), want)      # strided rows
+    odd = torch.zeros(6, k + 1, dtype=x.dtype, device=DEV)
+    odd[:, 1:] = x
+    assert torch.equal(ops.nvfp4_linear(odd[:, 1:], packed, scales, s2, bias), want)       # unaligned: copied
+    assert torch.equal(ops.nvfp4_linear(x[:1].expand(6, k), packed, scales, s2, bias), want[:1].expand(6, n))
+    assert ops.nvfp4_linear(x[:0], packed, scales, s2).shape == (0, n)
+    shifted = torch.empty(n * k // 2 + 1, dtype=torch.uint8, device=DEV)[1:].view(n, k // 2)
+    shifted.copy_(packed)
+    assert torch.equal(ops.nvfp4_linear(x, shifted, scales, s2, bias), want)
+
+
+@pytest.mark.parametrize("scale", [1e-36, 1e-5, 1e5, 1e36])
+def test_bf16_rows_of_any_magnitude(scale):
+    from b200q import ops
+
+    packed, scales, s2, w = _nvfp4(40, 1024, torch.bfloat16, seed=1)
+    x = (_x(5, 1024, torch.bfloat16).float() * scale).bfloat16()
+    x[1] *= 2.0 ** -60 if scale > 1 else 1                 # rows are scaled one by one
+    assert torch.isfinite(x).all()
+    _close(ops.nvfp4_linear(x, packed, scales, s2), x, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_not_finite_rows_stay_alone(dtype):
+    from b200q import ops
+
+    packed, scales, w = _int4(64, 512, 128, dtype, seed=4)
+    x = _x(9, 512, dtype)
+    want = ops.int4_linear(x, packed, scales, 128)
+    y = x.clone()
+    y[2, 77], y[8, 500] = math.inf, math.nan
+    got = ops.int4_linear(y, packed, scales, 128)
+    keep = [0, 1, 3, 4, 5, 6, 7]
+    assert torch.equal(got[keep], want[keep])
+    assert torch.isnan(got[8]).all()
+    zero = w[:, 77] == 0
+    assert torch.isnan(got[2][zero]).all()                # inf * 0
+    assert torch.equal(got[2][~zero], torch.copysign(torch.full_like(got[2], math.inf), w[:, 77].to(dtype))[~zero])
+
+
+def test_zero_blocks_and_zero_rows():
+    from b200q import ops
+
+    w = torch.randn(20, 256, device=DEV).bfloat16()
+    w[3], w[5, :128] = 0, 0
+    packed, scales = ops.int4_quantize(w.reshape(-1), 128)                 # 7 / 0 = inf: the block's weights are 0
+    x = _x(4, 256, torch.bfloat16)
+    x[2] = 0
+    out = ops.int4_linear(x, packed.view(20, 128), scales, 128)
+    assert torch.isfinite(out).all() and (out[:, 3] == 0).all() and (out[2] == 0).all()
+
+
+def test_deterministic_and_on_two_streams():
+    from b200q import ops
+
+    packed, scales, s2, _ = _nvfp4(512, 8192, torch.bfloat16, seed=1)
+    xs = [_x(16, 8192, torch.bfloat16, s) for s in range(2)]
+    want = [ops.nvfp4_linear(x, packed, scales, s2) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.nvfp4_linear(xs[i], packed, scales, s2))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_captured_and_replayed():
+    from b200q import ops
+
+    packed, scales, w = _int4(300, 1024, 64, torch.float16, seed=2)
+    x = _x(3, 1024, torch.float16, 1)
+    ops.int4_linear(x, packed, scales, 64)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.int4_linear(x, packed, scales, 64)
+    for seed in (5, 6):
+        x.copy_(_x(3, 1024, torch.float16, seed))
+        graph.replay()
+        assert torch.equal(out, ops.int4_linear(x, packed, scales, 64))
+
+
+def test_refusals():
+    from b200q import ops
+
+    packed, scales, w = _int4(16, 256, 128, torch.float16, seed=2)
+    x = _x(2, 256, torch.float16)
+    with pytest.raises(TypeError):
+        ops.int4_linear(x.float(), packed, scales.float(), 128)
+    with pytest.raises(TypeError):
+        ops.int4_linear(x, packed, scales.bfloat16(), 128)
+    for args in ((x[:, :128], packed, scales, 128), (x, packed, scales[:5], 128), (x, packed, scales, 64), (x, packed, scales, 16),
+                 (x, packed, scales, 96), (x, packed.view(-1), scales, 128), (x, packed, scales, 128, torch.zeros(3, device=DEV))):
+        with pytest.raises(ValueError):
+            ops.int4_linear(*args)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.int4_linear(x.cpu(), packed, scales, 128)
+    with pytest.raises(TypeError):
+        ops.nvfp4_linear(x, packed, scales, torch.ones((), device=DEV))
+    assert not ops.w4_linear_supported(x[:, :16], 16, 16)
