@@ -18,14 +18,19 @@
 // and walks over the row tiles with its part of x resident in shared memory.  Each lane fetches its own operands
 // with cp.async into a ring (kStages x 1 KB a warp, so 96 KB in flight on an SM), which runs on across tiles.
 // Partial sums meet in shared memory, across the cluster through distributed shared memory, in a fixed order.
+#include <atomic>
+
 #include "umma.cuh"
 
 namespace b200q {
 
-constexpr int kW4Warps = 8, kW4Threads = 32 * kW4Warps;
+constexpr int kW4Warps = 16, kW4Threads = 32 * kW4Warps;
 constexpr int kW4Rows = 16;                  // weight rows of a tile
 constexpr int kSlab = 128;                   // k elements a warp handles at a time
-constexpr int kW4Stages = 6;
+#ifndef W4ST
+#define W4ST 5
+#endif
+constexpr int kW4Stages = W4ST;
 
 struct W4Args {
   const void* x;
@@ -37,7 +42,7 @@ struct W4Args {
   void* out;                                 // [rows, n]
   int64_t out_stride;
   int rows, n, k, groups, group_slabs;       // groups a row; slabs a group (groups of 128 and more)
-  int slabs_per_cta, tiles;
+  int slabs_per_cta, tiles, wk, ks;
 };
 
 __device__ __forceinline__ uint32_t w4_pack_f16(float lo, float hi) {
@@ -92,49 +97,49 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float r;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
-  return r;
-}
-
 enum { kFmtInt4 = 0, kFmtNvfp4 = 1 };
 
 // LW: words (of 8 codes) in a lane's contiguous run.  Lane qd of a quad holds the elements
 //   slab * 128 + (i / LW) * 32 LW + qd * 8 LW + 8 (i % LW) + 0..7   for i = 0..3,
 // so that an instruction's 16 elements always lie in one group of 32 LW (INT4 groups of 32, 64, 128 n).
 template <int FMT, typename T, int NT, int LW>
-__global__ void __launch_bounds__(kW4Threads, 2)
+__global__ void __launch_bounds__(kW4Threads, 1)
 w4_linear_kernel(const W4Args a) {
   constexpr int kSegs = 4 / LW;                     // groups a slab has (at least)
   constexpr int kRunBytes = 4 * LW;
   constexpr int kPart = kW4Rows * 8 * NT;           // partial sums of a warp
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t xmax[8 * NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
-  uint32_t ks = 1, rank = 0;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ks));
-  rank = cluster_ctarank();
+  const int ks = a.ks, wk = a.wk, wr = kW4Warps / wk;
+  const int rank = static_cast<int>(cluster_ctarank());
   const int cluster = blockIdx.x / ks, nclusters = gridDim.x / ks;
   const int slab0 = rank * a.slabs_per_cta;
   const int slabs = max(min(a.slabs_per_cta, (a.k + kSlab - 1) / kSlab - slab0), 0);
+  const int my_row = warp / wk, my_k = warp % wk;   // which of the CTA's tiles, which part of its slabs
 
-  float* part = reinterpret_cast<float*>(smem);                                   // [2][warps][16][8 NT]
-  uint8_t* ring = smem + 2 * kW4Warps * kPart * 4 + warp * kW4Stages * 1024;      // [stages][2][32 lanes][16 B]
-  uint8_t* xs = smem + 2 * kW4Warps * kPart * 4 + kW4Warps * kW4Stages * 1024;    // [slab][i][qd][row] 16 B
+  uint8_t* ring = smem + warp * kW4Stages * 1024;   // [stages][2][32 lanes][16 B]
+  uint8_t* xs = smem + kW4Warps * kW4Stages * 1024; // [slab][i][qd][row] 16 B
+  float* part = reinterpret_cast<float*>(xs + static_cast<int64_t>(a.slabs_per_cta) * kSlab * 2 * a.rows);   // [warps][8 NT][16], wk > 1
+  float* recv = part + (wk > 1 ? kW4Warps * kPart : 0);                           // [ks][wr * 16 * rows / ks], ks > 1
   const uint32_t ring_addr = smem_u32(ring) + lane * 16;
 
   pdl_prologue();
 
-  // ---- producer: this lane's operands of one slab of one tile ----
-  const int mine = slabs > warp ? (slabs - warp + kW4Warps - 1) / kW4Warps : 0;   // slabs of this warp in each tile
-  const int my_tiles = a.tiles > cluster ? (a.tiles - cluster + nclusters - 1) / nclusters : 0;
+  // tiles of round t: (t * wr + my_row) * nclusters + cluster, so that the last round is spread over the SMs
+  const int mine = slabs > my_k ? (slabs - my_k + wk - 1) / wk : 0;               // slabs of this warp in each tile
+  const int first_tile = my_row * nclusters + cluster, tile_step = wr * nclusters;
+  const int rounds = (a.tiles - cluster + tile_step - 1) / tile_step;             // of the CTA
+  const int my_tiles = a.tiles > first_tile ? (a.tiles - first_tile + tile_step - 1) / tile_step : 0;
+  const int steps = mine * my_tiles;
   const int64_t row_bytes = a.k / 2;
-  int p_tile = cluster, p_i = 0, p_stage = 0;
-  int p_left = mine * my_tiles;
+
+  // ---- producer: this lane's operands of one slab of one tile ----
+  int p_tile = first_tile, p_i = 0, p_stage = 0, p_left = steps;
   auto produce = [&]() {
     if (p_left > 0) {
-      const int slab = slab0 + warp + p_i * kW4Warps;
+      const int slab = slab0 + my_k + p_i * wk;
       const int r0 = min(p_tile * kW4Rows + gr, a.n - 1), r1 = min(p_tile * kW4Rows + gr + 8, a.n - 1);
 #pragma unroll
       for (int seg = 0; seg < kSegs; ++seg) {
@@ -146,13 +151,39 @@ w4_linear_kernel(const W4Args a) {
         }
       }
       --p_left;
-      if (++p_i == mine) { p_i = 0; p_tile += nclusters; }
+      if (++p_i == mine) { p_i = 0; p_tile += tile_step; }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
   };
 #pragma unroll 1
   for (int s = 0; s < kW4Stages - 1; ++s) produce();
+
+  // ---- scales, one slab ahead of their use ----
+  constexpr int kScales = FMT == kFmtInt4 ? kSegs : 1;
+  using Raw = typename std::conditional<FMT == kFmtInt4, T, uint16_t>::type;      // INT4: a group's scale; NVFP4: two E4M3
+  Raw nxt[2][kScales];
+  int s_tile = first_tile, s_i = 0, s_left = steps;
+  auto load_scales = [&]() {
+    if (s_left > 0) {
+      const int slab = slab0 + my_k + s_i * wk;
+      const int64_t r0 = min(s_tile * kW4Rows + gr, a.n - 1), r1 = min(s_tile * kW4Rows + gr + 8, a.n - 1);
+#pragma unroll
+      for (int seg = 0; seg < kScales; ++seg) {
+        int64_t at;
+        if constexpr (FMT == kFmtInt4) at = LW == 4 ? slab / a.group_slabs : slab * kSegs + seg;
+        else at = slab * (kSlab / 16) + 2 * qd;
+        at = min(at, static_cast<int64_t>(a.groups) - (FMT == kFmtInt4 ? 1 : 2));  // behind the end of a row x is zero
+        const uint8_t* s = static_cast<const uint8_t*>(a.scales);
+        constexpr int kSize = FMT == kFmtInt4 ? 2 : 1;
+        nxt[0][seg] = __ldg(reinterpret_cast<const Raw*>(s + (r0 * a.groups + at) * kSize));
+        nxt[1][seg] = __ldg(reinterpret_cast<const Raw*>(s + (r1 * a.groups + at) * kSize));
+      }
+      --s_left;
+      if (++s_i == mine) { s_i = 0; s_tile += tile_step; }
+    }
+  };
+  load_scales();
 
   // ---- x into shared memory, as fp16 times a power of two ----
   const int packs = slabs * (kSlab / 8);            // 16-byte units a row
@@ -161,13 +192,15 @@ w4_linear_kernel(const W4Args a) {
   auto load_x = [&](int row, int p) {
     return k0 + 8 * p < a.k ? *reinterpret_cast<const uint4*>(x + row * a.x_stride + k0 + 8 * p) : make_uint4(0, 0, 0, 0);
   };
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+  if constexpr (kBf16) {
     if (threadIdx.x < 8 * NT) xmax[threadIdx.x] = 0;
     __syncthreads();
-    for (int row = 0; row < a.rows; ++row) {
-      uint32_t top = 0;                             // largest finite |x|, as a bf16 pattern
+    const int segs = (packs + 31) / 32;             // a warp reads 32 units of a row
 #pragma unroll 4
-      for (int p = threadIdx.x; p < packs; p += kW4Threads) {
+    for (int u = warp; u < a.rows * segs; u += kW4Warps) {
+      const int row = u / segs, p = (u - row * segs) * 32 + lane;
+      uint32_t top = 0;                             // largest finite |x|, as a bf16 pattern
+      if (p < packs) {
         const uint4 v = load_x(row, p);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -181,33 +214,37 @@ w4_linear_kernel(const W4Args a) {
     }
     __syncthreads();
   }
-  for (int row = 0; row < a.rows; ++row) {
-    float up = 1.f;
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-      up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - max(static_cast<int>(xmax[row] >> 7), 28)) << 23);
+  {
+    // neighbouring lanes take neighbouring rows (up to eight): their units are neighbours in shared memory
+    const int side = a.rows >= 8 ? 8 : a.rows >= 4 ? 4 : a.rows >= 2 ? 2 : 1;
+    const int wide = 32 / side, psegs = (packs + wide - 1) / wide, rgroups = (a.rows + side - 1) / side;
 #pragma unroll 4
-    for (int p = threadIdx.x; p < packs; p += kW4Threads) {
-      const uint4 v = load_x(row, p);
-      uint32_t h[4] = {v.x, v.y, v.z, v.w};
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    for (int u = warp; u < rgroups * psegs; u += kW4Warps) {
+      const int rg = u / psegs, p = (u - rg * psegs) * wide + lane / side, row = rg * side + lane % side;
+      if (p < packs && row < a.rows) {
+        const uint4 v = load_x(row, p);
+        uint32_t h[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (kBf16) {
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - max(static_cast<int>(xmax[row] >> 7), 28)) << 23);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
+          for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
+        }
+        uint4 o;
+        if constexpr (FMT == kFmtInt4) {            // (1, 5), (0, 4), (3, 7), (2, 6)
+          o.x = __byte_perm(h[0], h[2], 0x7632);
+          o.y = __byte_perm(h[0], h[2], 0x5410);
+          o.z = __byte_perm(h[1], h[3], 0x7632);
+          o.w = __byte_perm(h[1], h[3], 0x5410);
+        } else {
+          o = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        const int slab = p / 16, r = p % 16;        // unit r of the slab is word i of lane q
+        const int seg = r / (4 * LW), q = (r % (4 * LW)) / LW, i = seg * LW + r % LW;
+        *reinterpret_cast<uint4*>(xs + (static_cast<int64_t>((slab * 4 + i) * 4 + q) * a.rows + row) * 16) = o;
       }
-      uint4 o;
-      if constexpr (FMT == kFmtInt4) {              // (1, 5), (0, 4), (3, 7), (2, 6)
-        o.x = __byte_perm(h[0], h[2], 0x7632);
-        o.y = __byte_perm(h[0], h[2], 0x5410);
-        o.z = __byte_perm(h[1], h[3], 0x7632);
-        o.w = __byte_perm(h[1], h[3], 0x5410);
-      } else {
-        o = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      const int slab = p / 16, r = p % 16;          // unit r of the slab is word i of lane q
-      const int seg = r / (4 * LW), q = (r % (4 * LW)) / LW, i = seg * LW + r % LW;
-      *reinterpret_cast<uint4*>(xs + ((static_cast<int64_t>((slab * 4 + i) * 4 + q)) * a.rows + row) * 16) = o;
     }
   }
-  __syncthreads();
+  if (ks > 1) cluster_barrier(); else __syncthreads();   // the others' shared memory may be written from here on
 
   float back[NT][2];                                // of the columns this thread's sums belong to
   const float s2 = FMT == kFmtNvfp4 ? __ldg(a.scale2) : 1.f;
@@ -216,43 +253,41 @@ w4_linear_kernel(const W4Args a) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = 8 * n + 2 * qd + j;
-      back[n][j] = 1.f;
-      if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        if (row < a.rows) back[n][j] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(xmax[row] >> 7), 28) - 14) << 23);
+      back[n][j] = s2;
+      if constexpr (kBf16)
+        if (row < a.rows) back[n][j] *= __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(xmax[row] >> 7), 28) - 14) << 23);
     }
 
-  int stage = 0, buf = 0;
-  for (int tile = cluster; tile < a.tiles; tile += nclusters) {
-    const int r0 = min(tile * kW4Rows + gr, a.n - 1), r1 = min(tile * kW4Rows + gr + 8, a.n - 1);
+  auto store = [&](int row, int col, float sum) {
+    if (col >= a.n) return;
+    if (a.bias) sum += Elem<T>::to_float(static_cast<const T*>(a.bias)[col]);
+    static_cast<T*>(a.out)[row * a.out_stride + col] = Elem<T>::from_float(sum);
+  };
+
+  int stage = 0;
+#pragma unroll 1
+  for (int round = 0; round < rounds; ++round) {
+    const int tile = first_tile + round * tile_step;
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    const int todo = tile < a.tiles ? mine : 0;
 #pragma unroll 1
-    for (int it = 0; it < mine; ++it) {
-      const int sl = warp + it * kW4Warps, slab = slab0 + sl;
-      // scales of this slab (the codes are in flight or here already)
-      float inv[2][kSegs];
-      uint32_t sc[2][2];
-      if constexpr (FMT == kFmtInt4) {
+    for (int it = 0; it < todo; ++it) {
+      const int sl = my_k + it * wk;
+      Raw cur[2][kScales];
 #pragma unroll
-        for (int seg = 0; seg < kSegs; ++seg) {
-          const int kk = slab * kSlab + seg * 32 * LW;
-          const int grp = LW == 4 ? slab / a.group_slabs : kk / (32 * LW);
-          const bool ok = kk < a.k;
-          const T* s = static_cast<const T*>(a.scales) + (ok ? grp : 0);
-          inv[0][seg] = ok ? Elem<T>::to_float(__ldg(s + static_cast<int64_t>(r0) * a.groups)) : INFINITY;
-          inv[1][seg] = ok ? Elem<T>::to_float(__ldg(s + static_cast<int64_t>(r1) * a.groups)) : INFINITY;
+      for (int seg = 0; seg < kScales; ++seg) { cur[0][seg] = nxt[0][seg]; cur[1][seg] = nxt[1][seg]; }
+      load_scales();
+      uint32_t sc[2][2];
+      if constexpr (FMT == kFmtNvfp4) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t h;
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(cur[r][0]));
+          sc[r][0] = __byte_perm(h, h, 0x1010);
+          sc[r][1] = __byte_perm(h, h, 0x3232);
         }
-      } else {
-        const int kk = slab * kSlab + 32 * qd;
-        const uint8_t* s = static_cast<const uint8_t*>(a.scales) + kk / 16;
-        const uint32_t u0 = kk < a.k ? __ldg(reinterpret_cast<const uint16_t*>(s + static_cast<int64_t>(r0) * a.groups)) : 0;
-        const uint32_t u1 = kk < a.k ? __ldg(reinterpret_cast<const uint16_t*>(s + static_cast<int64_t>(r1) * a.groups)) : 0;
-        uint32_t h0, h1;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h0) : "h"(static_cast<uint16_t>(u0)));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h1) : "h"(static_cast<uint16_t>(u1)));
-        sc[0][0] = __byte_perm(h0, h0, 0x1010); sc[0][1] = __byte_perm(h0, h0, 0x3232);
-        sc[1][0] = __byte_perm(h1, h1, 0x1010); sc[1][1] = __byte_perm(h1, h1, 0x3232);
       }
       asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages - 2) : "memory");
       const uint4 va = *reinterpret_cast<const uint4*>(ring + stage * 1024 + lane * 16);
@@ -281,7 +316,7 @@ w4_linear_kernel(const W4Args a) {
             w4_mma(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
             w4_mma(tmp[n], fa[2], fb[2], fa[3], fb[3], b.z, b.w);
             if (i % LW == LW - 1) {
-              const float i0 = rcp_approx(inv[0][i / LW]), i1 = rcp_approx(inv[1][i / LW]);
+              const float i0 = rcp_approx(Elem<T>::to_float(cur[0][i / LW])), i1 = rcp_approx(Elem<T>::to_float(cur[1][i / LW]));
               acc[n][0] += tmp[n][0] * i0; acc[n][1] += tmp[n][1] * i0;
               acc[n][2] += tmp[n][2] * i1; acc[n][3] += tmp[n][3] * i1;
             }
@@ -294,69 +329,91 @@ w4_linear_kernel(const W4Args a) {
       produce();                                    // into the slot read one slab ago
       stage = stage + 1 == kW4Stages ? 0 : stage + 1;
     }
-    // ---- partial sums of the warps and CTAs ----
-    float* mypart = part + (buf * kW4Warps + warp) * kPart;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        mypart[(gr + 8 * (j >> 1)) + kW4Rows * (8 * n + 2 * qd + (j & 1))] = acc[n][j] * (back[n][j & 1] * s2);
-    if (ks > 1) cluster_barrier(); else __syncthreads();
-    const int todo = kW4Rows * a.rows;
-    for (int e = rank * kW4Threads + threadIdx.x; e < todo; e += ks * kW4Threads) {
-      const int wr = e % kW4Rows, row = e / kW4Rows, col = tile * kW4Rows + wr;
-      float sum = 0.f;
-      if (ks == 1) {
+      for (int j = 0; j < 4; ++j) acc[n][j] *= back[n][j & 1];
+
+    // ---- sums of the K parts, always in the order of the warps and CTAs ----
+    const int elems = kW4Rows * a.rows;             // of a tile
+    const int per = wr * elems / ks;                // of the CTA's tiles that one CTA of the cluster finishes
+    auto push = [&](int e, float v) {               // element e of the CTA's tiles to the CTA that finishes it
+      const uint32_t to = map_to_cta(recv + rank * per + e % per, e / per);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+    };
+    if (wk > 1) {
+      float* p = part + warp * kPart;
 #pragma unroll
-        for (int w = 0; w < kW4Warps; ++w) sum += part[(buf * kW4Warps + w) * kPart + e];
-      } else {
-        for (uint32_t c = 0; c < ks; ++c) {
-          const uint32_t base = map_to_cta(part + buf * kW4Warps * kPart + e, c);
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int w = 0; w < kW4Warps; ++w) sum += ld_cluster_f32(base + w * kPart * 4);
+        for (int j = 0; j < 4; ++j) p[gr + 8 * (j >> 1) + kW4Rows * (8 * n + 2 * qd + (j & 1))] = acc[n][j];
+      __syncthreads();
+      for (int e = threadIdx.x; e < wr * elems; e += kW4Threads) {
+        const int t = e / elems, in = e - t * elems;
+        float sum = 0.f;
+        for (int w = 0; w < wk; ++w) sum += part[(t * wk + w) * kPart + in];
+        if (ks > 1) push(e, sum);
+        else store(in / kW4Rows, (first_tile - my_row * nclusters + round * tile_step + t * nclusters) * kW4Rows + in % kW4Rows, sum);
+      }
+      if (ks == 1) __syncthreads();                 // read before the next round writes
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int wrow = gr + 8 * (j >> 1), row = 8 * n + 2 * qd + (j & 1);
+          if (row >= a.rows) continue;
+          if (ks > 1) push(my_row * elems + row * kW4Rows + wrow, acc[n][j]);
+          else if (tile < a.tiles) store(row, tile * kW4Rows + wrow, acc[n][j]);
         }
-      }
-      if (col < a.n) {
-        if (a.bias) sum += Elem<T>::to_float(static_cast<const T*>(a.bias)[col]);
-        static_cast<T*>(a.out)[row * a.out_stride + col] = Elem<T>::from_float(sum);
-      }
     }
-    buf ^= 1;                                       // the other half: its readers passed the barrier above
+    if (ks > 1) {
+      cluster_barrier();
+      for (int i = threadIdx.x; i < per; i += kW4Threads) {
+        float sum = 0.f;
+        for (int c = 0; c < ks; ++c) sum += recv[c * per + i];
+        const int e = rank * per + i, t = e / elems, in = e - t * elems;
+        store(in / kW4Rows, (cluster + round * tile_step + t * nclusters) * kW4Rows + in % kW4Rows, sum);
+      }
+      if (round + 1 < rounds) cluster_barrier();    // read before the next round's sums arrive
+    }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (ks > 1) cluster_barrier();                    // nobody leaves while its partial sums may be read
 }
 
-// shared memory of a CTA that holds `rows` rows of x over `slabs` slabs
-inline size_t w4_smem(int rows, int nt, int slabs) {
-  return 2 * kW4Warps * kW4Rows * 8 * static_cast<size_t>(nt) * 4 + kW4Warps * kW4Stages * 1024 +
-         static_cast<size_t>(slabs) * kSlab * 2 * rows;
+inline size_t w4_smem(int rows, int nt, int slabs, int wk, int ks) {
+  return kW4Warps * kW4Stages * 1024 + static_cast<size_t>(slabs) * kSlab * 2 * rows +
+         (wk > 1 ? kW4Warps * kW4Rows * 8 * 4 * static_cast<size_t>(nt) : 0) +
+         (ks > 1 ? static_cast<size_t>(kW4Warps / wk) * kW4Rows * 4 * rows : 0);
 }
 constexpr size_t kW4SmemLimit = 227 * 1024 - 1024;
+inline int w4_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
+// How K is cut: over the wk warps of a tile and the ks CTAs of a cluster.  x decides the least ks (its part has to fit
+// beside the ring); then wk and after it ks grow until every warp of the GPU has a tile part, while a part keeps two slabs.
+inline bool w4_cut(int rows, int slabs, int tiles, int sms, int& wk, int& ks) {
+  const int nt = w4_nt(rows);
+  for (ks = 1; ks < 8 && w4_smem(rows, nt, (slabs + ks - 1) / ks, 1, ks) > kW4SmemLimit; ks *= 2) {}
+  wk = 1;
+  auto fits = [&](int w, int c) { return w4_smem(rows, nt, (slabs + c - 1) / c, w, c) <= kW4SmemLimit; };
+  if (!fits(1, ks)) return false;
+  auto more = [&] { return static_cast<int64_t>(tiles) * wk * ks * 4 < 3ll * sms * kW4Warps && slabs >= 4 * wk * ks; };
+  while (wk < kW4Warps && more() && fits(2 * wk, ks)) wk *= 2;
+  while (ks < 8 && more() && fits(wk, 2 * ks)) ks *= 2;
+  return true;
+}
 
 template <int FMT, typename T, int NT, int LW>
 int launch_w4(W4Args a, cudaStream_t s) {
   auto kern = w4_linear_kernel<FMT, T, NT, LW>;
-  const int slabs = (a.k + kSlab - 1) / kSlab;
-  // K over 1, 2, 4 or 8 CTAs: until two CTAs fit an SM and every SM has two, while each warp keeps a slab
-  int ks = 1;
-  const int sms = sm_count_cached();
-  while (ks < 8) {
-    const size_t need = w4_smem(a.rows, NT, (slabs + ks - 1) / ks);
-    const bool fits = need <= kW4SmemLimit / 2;
-    const bool full = static_cast<int64_t>(a.tiles) * ks >= 2 * sms;
-    if ((fits && full) || (need <= kW4SmemLimit && slabs / (2 * ks) < kW4Warps)) break;
-    ks *= 2;
-  }
-  a.slabs_per_cta = (slabs + ks - 1) / ks;
-  const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta);
-  if (smem > kW4SmemLimit) return B200Q_ERR_CAPACITY;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+  const int slabs = (a.k + kSlab - 1) / kSlab, sms = sm_count_cached();
+  if (!w4_cut(a.rows, slabs, a.tiles, sms, a.wk, a.ks)) return B200Q_ERR_CAPACITY;
+  a.slabs_per_cta = (slabs + a.ks - 1) / a.ks;
+  const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, a.wk, a.ks);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kW4SmemLimit)) != cudaSuccess)
     return B200Q_ERR_CUDA;
-  const int per_sm = smem <= kW4SmemLimit / 2 ? 2 : 1;
-  const int clusters = max(1, min(a.tiles, sms * per_sm / ks));
+  const int wr = kW4Warps / a.wk;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters * ks));
   cfg.blockDim = dim3(kW4Threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -364,10 +421,24 @@ int launch_w4(W4Args a, cudaStream_t s) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(ks);
+  attr[1].val.clusterDim.x = static_cast<unsigned>(a.ks);
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
+  int room = sms / a.ks;                            // clusters the GPU holds at a time (they need SMs of one GPC)
+  if (a.ks > 2) {
+    static std::atomic<int> cached[2];              // clusters of 4, of 8; every block has an SM to itself
+    int c = cached[a.ks == 4 ? 0 : 1];
+    if (c == 0) {
+      int got = 0;
+      cfg.gridDim = dim3(static_cast<unsigned>(room * a.ks));
+      if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) == cudaSuccess && got > 0)
+        cached[a.ks == 4 ? 0 : 1] = c = got;
+    }
+    if (c > 0) room = min(room, c);
+  }
+  const int clusters = max(1, min((a.tiles + wr - 1) / wr, room));
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * a.ks));
   cudaLaunchKernelEx(&cfg, kern, a);
   return launch_status();
 }
@@ -413,9 +484,9 @@ using namespace b200q;
 
 extern "C" int b200q_w4_linear_max_rows(int64_t k) {
   if (k <= 0 || k % 32 || k > (1 << 24)) return 0;
-  const int slabs = static_cast<int>((k + kSlab - 1) / kSlab), part = (slabs + 7) / 8;
+  const int slabs = static_cast<int>((k + kSlab - 1) / kSlab);
   for (int rows = 32; rows > 0; --rows)
-    if (w4_smem(rows, rows <= 8 ? 1 : rows <= 16 ? 2 : 4, part) <= kW4SmemLimit) return rows;
+    if (w4_smem(rows, w4_nt(rows), (slabs + 7) / 8, 1, 8) <= kW4SmemLimit) return rows;
   return 0;
 }
 
