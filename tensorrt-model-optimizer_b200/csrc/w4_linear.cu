@@ -28,9 +28,10 @@ constexpr int kW4Warps = 16, kW4Threads = 32 * kW4Warps;
 constexpr int kW4Rows = 16;                  // weight rows of a tile
 constexpr int kSlab = 128;                   // k elements a warp handles at a time
 #ifndef W4ST
-#define W4ST 5
+#define W4ST 3
 #endif
-constexpr int kW4Stages = W4ST;
+constexpr int kW4Stages = W4ST;               // of two slabs
+constexpr int kStageBytes = 2048;
 
 struct W4Args {
   const void* x;
@@ -43,6 +44,7 @@ struct W4Args {
   int64_t out_stride;
   int rows, n, k, groups, group_slabs;       // groups a row; slabs a group (groups of 128 and more)
   int slabs_per_cta, tiles, wk, ks;
+  FastDiv pairs;                             // slab pairs of a CTA
 };
 
 __device__ __forceinline__ uint32_t w4_pack_f16(float lo, float hi) {
@@ -54,6 +56,12 @@ __device__ __forceinline__ void w4_mma(float* c, uint32_t a0, uint32_t a1, uint3
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same with a zero accumulator
+__device__ __forceinline__ void w4_mma_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 template <int N>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
@@ -94,7 +102,7 @@ __device__ __forceinline__ uint32_t w4_hmul2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ float rcp_approx(float x) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 enum { kFmtInt4 = 0, kFmtNvfp4 = 1 };
@@ -119,131 +127,168 @@ w4_linear_kernel(const W4Args a) {
   const int slabs = max(min(a.slabs_per_cta, (a.k + kSlab - 1) / kSlab - slab0), 0);
   const int my_row = warp / wk, my_k = warp % wk;   // which of the CTA's tiles, which part of its slabs
 
-  uint8_t* ring = smem + warp * kW4Stages * 1024;   // [stages][2][32 lanes][16 B]
-  uint8_t* xs = smem + kW4Warps * kW4Stages * 1024; // [slab][i][qd][row] 16 B
-  float* part = reinterpret_cast<float*>(xs + static_cast<int64_t>(a.slabs_per_cta) * kSlab * 2 * a.rows);   // [warps][8 NT][16], wk > 1
+  uint8_t* ring = smem + warp * kW4Stages * kStageBytes;      // [stages][2 slabs][2 rows][32 lanes][16 B]
+  uint8_t* xs = smem + kW4Warps * kW4Stages * kStageBytes; // [slab][i][row][qd] 16 B
+  float* part = reinterpret_cast<float*>(xs + static_cast<int64_t>(a.pairs.d) * 2 * kSlab * 2 * a.rows);   // [warps][8 NT][16], wk > 1
   float* recv = part + (wk > 1 ? kW4Warps * kPart : 0);                           // [ks][wr * 16 * rows / ks], ks > 1
   const uint32_t ring_addr = smem_u32(ring) + lane * 16;
 
   pdl_prologue();
 
   // tiles of round t: (t * wr + my_row) * nclusters + cluster, so that the last round is spread over the SMs
-  const int mine = slabs > my_k ? (slabs - my_k + wk - 1) / wk : 0;               // slabs of this warp in each tile
+  const int npairs = (slabs + 1) / 2;
+  const int mine = npairs > my_k ? (npairs - my_k + wk - 1) / wk : 0;             // slab pairs of this warp in each tile
   const int first_tile = my_row * nclusters + cluster, tile_step = wr * nclusters;
   const int rounds = (a.tiles - cluster + tile_step - 1) / tile_step;             // of the CTA
   const int my_tiles = a.tiles > first_tile ? (a.tiles - first_tile + tile_step - 1) / tile_step : 0;
   const int steps = mine * my_tiles;
   const int64_t row_bytes = a.k / 2;
 
-  // ---- producer: this lane's operands of one slab of one tile ----
-  int p_tile = first_tile, p_i = 0, p_stage = 0, p_left = steps;
+  // ---- producer: this lane's operands of two slabs of one tile ----
+  // Addresses are kept as pointers that step through a tile's slabs: the arithmetic of an address from
+  // scratch costs as many issue slots as the conversions.
+  const int slab_first = slab0 + 2 * my_k;
+  const int code_step = wk * kSlab;
+  auto row_of = [&](int tile, int r) { return static_cast<int64_t>(min(tile * kW4Rows + gr + 8 * r, a.n - 1)); };
+  const int64_t code_first = slab_first * (kSlab / 2) + qd * kRunBytes;
+  const uint8_t *pc0 = a.codes, *pc1 = a.codes;
+  int p_tile = first_tile, p_i = 0, p_left = steps, p_k = 0;
+  uint32_t p_dst = ring_addr;
   auto produce = [&]() {
     if (p_left > 0) {
-      const int slab = slab0 + my_k + p_i * wk;
-      const int r0 = min(p_tile * kW4Rows + gr, a.n - 1), r1 = min(p_tile * kW4Rows + gr + 8, a.n - 1);
+      if (p_i == 0) {
+        pc0 = a.codes + row_of(p_tile, 0) * row_bytes + code_first;
+        pc1 = a.codes + row_of(p_tile, 1) * row_bytes + code_first;
+        p_k = slab_first * kSlab + qd * 8 * LW;
+        p_tile += tile_step;
+      }
 #pragma unroll
-      for (int seg = 0; seg < kSegs; ++seg) {
-        const int kk = slab * kSlab + seg * 32 * LW + qd * 8 * LW;
-        if (kk < a.k) {
-          const uint32_t dst = ring_addr + p_stage * 1024 + seg * kRunBytes;
-          copy_async<kRunBytes>(dst, a.codes + r0 * row_bytes + kk / 2);
-          copy_async<kRunBytes>(dst + 512, a.codes + r1 * row_bytes + kk / 2);
+      for (int seg = 0; seg < 2 * kSegs; ++seg) {
+        const uint32_t to = p_dst + (seg / kSegs) * 1024 + (seg % kSegs) * kRunBytes;
+        if (p_k + seg * 32 * LW < a.k) {
+          copy_async<kRunBytes>(to, pc0 + seg * 16 * LW);
+          copy_async<kRunBytes>(to + 512, pc1 + seg * 16 * LW);
         }
       }
+      pc0 += code_step;
+      pc1 += code_step;
+      p_k += 2 * code_step;
+      p_i = p_i + 1 == mine ? 0 : p_i + 1;
       --p_left;
-      if (++p_i == mine) { p_i = 0; p_tile += tile_step; }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
   };
 #pragma unroll 1
-  for (int s = 0; s < kW4Stages - 1; ++s) produce();
+  for (int s = 0; s < kW4Stages - 1; ++s) {
+    p_dst = ring_addr + s * kStageBytes;
+    produce();
+  }
 
-  // ---- scales, one slab ahead of their use ----
-  constexpr int kScales = FMT == kFmtInt4 ? kSegs : 1;
+  // ---- scales, two slabs ahead of their use ----
+  constexpr int kScales = FMT == kFmtInt4 ? 2 * kSegs : 2;                        // of a row in two slabs
+  constexpr int kScaleSize = FMT == kFmtInt4 ? 2 : 1;
   using Raw = typename std::conditional<FMT == kFmtInt4, T, uint16_t>::type;      // INT4: a group's scale; NVFP4: two E4M3
   Raw nxt[2][kScales];
-  int s_tile = first_tile, s_i = 0, s_left = steps;
+  const uint8_t *ps0 = nullptr, *ps1 = nullptr;     // the row's scales
+  int s_tile = first_tile, s_i = 0, s_left = steps, s_at = 0;
   auto load_scales = [&]() {
     if (s_left > 0) {
-      const int slab = slab0 + my_k + s_i * wk;
-      const int64_t r0 = min(s_tile * kW4Rows + gr, a.n - 1), r1 = min(s_tile * kW4Rows + gr + 8, a.n - 1);
+      if (s_i == 0) {
+        ps0 = static_cast<const uint8_t*>(a.scales) + row_of(s_tile, 0) * a.groups * kScaleSize;
+        ps1 = static_cast<const uint8_t*>(a.scales) + row_of(s_tile, 1) * a.groups * kScaleSize;
+        s_at = FMT == kFmtInt4 ? slab_first * kSegs : slab_first * (kSlab / 16) + 2 * qd;
+        s_tile += tile_step;
+      }
 #pragma unroll
       for (int seg = 0; seg < kScales; ++seg) {
-        int64_t at;
-        if constexpr (FMT == kFmtInt4) at = LW == 4 ? slab / a.group_slabs : slab * kSegs + seg;
-        else at = slab * (kSlab / 16) + 2 * qd;
-        at = min(at, static_cast<int64_t>(a.groups) - (FMT == kFmtInt4 ? 1 : 2));  // behind the end of a row x is zero
-        const uint8_t* s = static_cast<const uint8_t*>(a.scales);
-        constexpr int kSize = FMT == kFmtInt4 ? 2 : 1;
-        nxt[0][seg] = __ldg(reinterpret_cast<const Raw*>(s + (r0 * a.groups + at) * kSize));
-        nxt[1][seg] = __ldg(reinterpret_cast<const Raw*>(s + (r1 * a.groups + at) * kSize));
+        int at = FMT == kFmtInt4 ? s_at + seg : s_at + seg * (kSlab / 16);
+        if (FMT == kFmtInt4 && LW == 4 && a.group_slabs > 1) at /= a.group_slabs;
+        at = min(at, a.groups - (FMT == kFmtInt4 ? 1 : 2));                        // behind the end of a row x is zero
+        nxt[0][seg] = __ldg(reinterpret_cast<const Raw*>(ps0 + at * kScaleSize));
+        nxt[1][seg] = __ldg(reinterpret_cast<const Raw*>(ps1 + at * kScaleSize));
       }
+      s_at += FMT == kFmtInt4 ? 2 * wk * kSegs : 2 * wk * (kSlab / 16);
+      s_i = s_i + 1 == mine ? 0 : s_i + 1;
       --s_left;
-      if (++s_i == mine) { s_i = 0; s_tile += tile_step; }
     }
   };
   load_scales();
 
   // ---- x into shared memory, as fp16 times a power of two ----
-  const int packs = slabs * (kSlab / 8);            // 16-byte units a row
+  // A warp takes two slabs of a row at a time; lane = 16 (slab) + 4 (word i) + q, so that the stores of eight lanes hit
+  // all banks (two at a time where the rows are even).  All loads are issued before the first is used; the maximum and
+  // the conversion both work on the registers.
+  constexpr int kHold = 18;                         // of 16 warps: all that shared memory has room for, almost
   const T* x = static_cast<const T*>(a.x);
-  const int k0 = slab0 * kSlab;
-  auto load_x = [&](int row, int p) {
-    return k0 + 8 * p < a.k ? *reinterpret_cast<const uint4*>(x + row * a.x_stride + k0 + 8 * p) : make_uint4(0, 0, 0, 0);
+  const int units = a.rows * static_cast<int>(a.pairs.d);
+  const int x_i = (lane >> 2) & 3, x_q = lane & 3;
+  const int x_k = slab0 * kSlab + (lane >> 4) * kSlab + ((x_i / LW) * 4 * LW + x_q * LW + x_i % LW) * 8;
+  auto load_x = [&](int u) {
+    uint32_t row, pair;
+    a.pairs.divmod(u, row, pair);
+    const int k = x_k + pair * (2 * kSlab);
+    return k < a.k ? __ldg(reinterpret_cast<const uint4*>(x + row * a.x_stride + k)) : make_uint4(0, 0, 0, 0);
   };
+  auto max_x = [&](int u, const uint4& v) {
+    uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    m = max(m & 0xffffu, m >> 16);
+    if (m >= 0x7f80u) {                             // infinity or NaN: the largest of the others
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      m = 0;
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
+        m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+      }
+    }
+    m = warp_max_u32(m);
+    if (lane == 0 && m) atomicMax(&xmax[a.pairs.div(u)], m);
+  };
+  auto store_x = [&](int u, const uint4& v) {
+    uint32_t row, pair;
+    a.pairs.divmod(u, row, pair);
+    const int slab = 2 * pair + (lane >> 4);
+    uint32_t h[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (kBf16) {
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - max(static_cast<int>(xmax[row] >> 7), 28)) << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
+    }
+    uint4 o;
+    if constexpr (FMT == kFmtInt4) {                // (1, 5), (0, 4), (3, 7), (2, 6)
+      o.x = __byte_perm(h[0], h[2], 0x7632);
+      o.y = __byte_perm(h[0], h[2], 0x5410);
+      o.z = __byte_perm(h[1], h[3], 0x7632);
+      o.w = __byte_perm(h[1], h[3], 0x5410);
+    } else {
+      o = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    *reinterpret_cast<uint4*>(xs + (((slab * 4 + x_i) * a.rows + static_cast<int>(row)) * 4 + x_q) * 16) = o;
+  };
+  uint4 hold[kHold];
+#pragma unroll
+  for (int j = 0; j < kHold; ++j) {
+    if (warp + j * kW4Warps >= units) break;
+    hold[j] = load_x(warp + j * kW4Warps);
+  }
   if constexpr (kBf16) {
     if (threadIdx.x < 8 * NT) xmax[threadIdx.x] = 0;
     __syncthreads();
-    const int segs = (packs + 31) / 32;             // a warp reads 32 units of a row
-#pragma unroll 4
-    for (int u = warp; u < a.rows * segs; u += kW4Warps) {
-      const int row = u / segs, p = (u - row * segs) * 32 + lane;
-      uint32_t top = 0;                             // largest finite |x|, as a bf16 pattern
-      if (p < packs) {
-        const uint4 v = load_x(row, p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
-          top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-        }
-      }
-      top = warp_max_u32(top);
-      if (lane == 0 && top) atomicMax(&xmax[row], top);
+    for (int j = 0; j < kHold; ++j) {
+      if (warp + j * kW4Warps >= units) break;
+      max_x(warp + j * kW4Warps, hold[j]);
     }
+#pragma unroll 1
+    for (int u = warp + kHold * kW4Warps; u < units; u += kW4Warps) max_x(u, load_x(u));
     __syncthreads();
   }
-  {
-    // neighbouring lanes take neighbouring rows (up to eight): their units are neighbours in shared memory
-    const int side = a.rows >= 8 ? 8 : a.rows >= 4 ? 4 : a.rows >= 2 ? 2 : 1;
-    const int wide = 32 / side, psegs = (packs + wide - 1) / wide, rgroups = (a.rows + side - 1) / side;
-#pragma unroll 4
-    for (int u = warp; u < rgroups * psegs; u += kW4Warps) {
-      const int rg = u / psegs, p = (u - rg * psegs) * wide + lane / side, row = rg * side + lane % side;
-      if (p < packs && row < a.rows) {
-        const uint4 v = load_x(row, p);
-        uint32_t h[4] = {v.x, v.y, v.z, v.w};
-        if constexpr (kBf16) {
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - max(static_cast<int>(xmax[row] >> 7), 28)) << 23);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
-        }
-        uint4 o;
-        if constexpr (FMT == kFmtInt4) {            // (1, 5), (0, 4), (3, 7), (2, 6)
-          o.x = __byte_perm(h[0], h[2], 0x7632);
-          o.y = __byte_perm(h[0], h[2], 0x5410);
-          o.z = __byte_perm(h[1], h[3], 0x7632);
-          o.w = __byte_perm(h[1], h[3], 0x5410);
-        } else {
-          o = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        const int slab = p / 16, r = p % 16;        // unit r of the slab is word i of lane q
-        const int seg = r / (4 * LW), q = (r % (4 * LW)) / LW, i = seg * LW + r % LW;
-        *reinterpret_cast<uint4*>(xs + (static_cast<int64_t>((slab * 4 + i) * 4 + q) * a.rows + row) * 16) = o;
-      }
-    }
+  for (int j = 0; j < kHold; ++j) {
+    if (warp + j * kW4Warps >= units) break;
+    store_x(warp + j * kW4Warps, hold[j]);
   }
+#pragma unroll 1
+  for (int u = warp + kHold * kW4Warps; u < units; u += kW4Warps) store_x(u, load_x(u));
   if (ks > 1) cluster_barrier(); else __syncthreads();   // the others' shared memory may be written from here on
 
   float back[NT][2];                                // of the columns this thread's sums belong to
@@ -264,7 +309,14 @@ w4_linear_kernel(const W4Args a) {
     static_cast<T*>(a.out)[row * a.out_stride + col] = Elem<T>::from_float(sum);
   };
 
-  int stage = 0;
+  uint32_t slot = 0;                                // ring offset of the slab at hand
+  p_dst = ring_addr + (kW4Stages - 1) * kStageBytes;
+  const uint8_t* lane_ring = ring + lane * 16;
+  // x of row 8 n + gr; columns beyond the last row repeat it, their sums are dropped
+  const uint8_t* lane_x[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) lane_x[n] = xs + (min(8 * n + gr, a.rows - 1) * 4 + qd) * 16;
+  const int word_step = 4 * a.rows * 16, slab_step = 4 * word_step;
 #pragma unroll 1
   for (int round = 0; round < rounds; ++round) {
     const int tile = first_tile + round * tile_step;
@@ -274,60 +326,67 @@ w4_linear_kernel(const W4Args a) {
     const int todo = tile < a.tiles ? mine : 0;
 #pragma unroll 1
     for (int it = 0; it < todo; ++it) {
-      const int sl = my_k + it * wk;
+      const uint8_t* xp[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) xp[n] = lane_x[n] + 2 * (my_k + it * wk) * slab_step;
       Raw cur[2][kScales];
 #pragma unroll
       for (int seg = 0; seg < kScales; ++seg) { cur[0][seg] = nxt[0][seg]; cur[1][seg] = nxt[1][seg]; }
       load_scales();
-      uint32_t sc[2][2];
-      if constexpr (FMT == kFmtNvfp4) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint32_t h;
-          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(cur[r][0]));
-          sc[r][0] = __byte_perm(h, h, 0x1010);
-          sc[r][1] = __byte_perm(h, h, 0x3232);
-        }
-      }
       asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages - 2) : "memory");
-      const uint4 va = *reinterpret_cast<const uint4*>(ring + stage * 1024 + lane * 16);
-      const uint4 vb = *reinterpret_cast<const uint4*>(ring + stage * 1024 + 512 + lane * 16);
-      const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
-      float tmp[NT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t fa[4], fb[4];
-        if constexpr (FMT == kFmtInt4) {
-          int4x8_to_f16(wa[i], fa);
-          int4x8_to_f16(wb[i], fb);
-        } else {
-          e2m1x8_to_f16(wa[i], fa);
-          e2m1x8_to_f16(wb[i], fb);
+      for (int half = 0; half < 2; ++half) {        // behind the end of K x is zero, and the codes whatever they are
+        const uint4 va = *reinterpret_cast<const uint4*>(lane_ring + slot + half * 1024);
+        const uint4 vb = *reinterpret_cast<const uint4*>(lane_ring + slot + half * 1024 + 512);
+        const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+        uint32_t sc[2][2];
+        if constexpr (FMT == kFmtNvfp4) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { fa[j] = w4_hmul2(fa[j], sc[0][i / 2]); fb[j] = w4_hmul2(fb[j], sc[1][i / 2]); }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint4 b = make_uint4(0, 0, 0, 0);
-          const int row = 8 * n + gr;
-          if (row < a.rows) b = *reinterpret_cast<const uint4*>(xs + (static_cast<int64_t>((sl * 4 + i) * 4 + qd) * a.rows + row) * 16);
-          if constexpr (FMT == kFmtInt4) {
-            if (i % LW == 0) tmp[n][0] = tmp[n][1] = tmp[n][2] = tmp[n][3] = 0.f;
-            w4_mma(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
-            w4_mma(tmp[n], fa[2], fb[2], fa[3], fb[3], b.z, b.w);
-            if (i % LW == LW - 1) {
-              const float i0 = rcp_approx(Elem<T>::to_float(cur[0][i / LW])), i1 = rcp_approx(Elem<T>::to_float(cur[1][i / LW]));
-              acc[n][0] += tmp[n][0] * i0; acc[n][1] += tmp[n][1] * i0;
-              acc[n][2] += tmp[n][2] * i1; acc[n][3] += tmp[n][3] * i1;
-            }
-          } else {
-            w4_mma(acc[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
-            w4_mma(acc[n], fa[2], fb[2], fa[3], fb[3], b.z, b.w);
+          for (int r = 0; r < 2; ++r) {
+            uint32_t h;
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(cur[r][half]));
+            sc[r][0] = __byte_perm(h, h, 0x1010);
+            sc[r][1] = __byte_perm(h, h, 0x3232);
           }
         }
+        float tmp[NT][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t fa[4], fb[4];
+          if constexpr (FMT == kFmtInt4) {
+            int4x8_to_f16(wa[i], fa);
+            int4x8_to_f16(wb[i], fb);
+          } else {
+            e2m1x8_to_f16(wa[i], fa);
+            e2m1x8_to_f16(wb[i], fb);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { fa[j] = w4_hmul2(fa[j], sc[0][i / 2]); fb[j] = w4_hmul2(fb[j], sc[1][i / 2]); }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 b = *reinterpret_cast<const uint4*>(xp[n] + i * word_step);
+            if constexpr (FMT == kFmtInt4) {
+              if (i % LW == 0) w4_mma_first(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
+              else w4_mma(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
+              w4_mma(tmp[n], fa[2], fb[2], fa[3], fb[3], b.z, b.w);
+              if (i % LW == LW - 1) {
+                const int seg = half * kSegs + i / LW;
+                const float i0 = rcp_approx(Elem<T>::to_float(cur[0][seg])), i1 = rcp_approx(Elem<T>::to_float(cur[1][seg]));
+                acc[n][0] += tmp[n][0] * i0; acc[n][1] += tmp[n][1] * i0;
+                acc[n][2] += tmp[n][2] * i1; acc[n][3] += tmp[n][3] * i1;
+              }
+            } else {
+              w4_mma(acc[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
+              w4_mma(acc[n], fa[2], fb[2], fa[3], fb[3], b.z, b.w);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) xp[n] += slab_step;
       }
-      produce();                                    // into the slot read one slab ago
-      stage = stage + 1 == kW4Stages ? 0 : stage + 1;
+      produce();                                    // into the slot read one step ago
+      p_dst = ring_addr + slot;
+      slot = slot == (kW4Stages - 1) * kStageBytes ? 0 : slot + kStageBytes;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -382,7 +441,7 @@ w4_linear_kernel(const W4Args a) {
 }
 
 inline size_t w4_smem(int rows, int nt, int slabs, int wk, int ks) {
-  return kW4Warps * kW4Stages * 1024 + static_cast<size_t>(slabs) * kSlab * 2 * rows +
+  return kW4Warps * kW4Stages * kStageBytes + static_cast<size_t>((slabs + 1) / 2 * 2) * kSlab * 2 * rows +
          (wk > 1 ? kW4Warps * kW4Rows * 8 * 4 * static_cast<size_t>(nt) : 0) +
          (ks > 1 ? static_cast<size_t>(kW4Warps / wk) * kW4Rows * 4 * rows : 0);
 }
@@ -408,11 +467,11 @@ int launch_w4(W4Args a, cudaStream_t s) {
   auto kern = w4_linear_kernel<FMT, T, NT, LW>;
   const int slabs = (a.k + kSlab - 1) / kSlab, sms = sm_count_cached();
   if (!w4_cut(a.rows, slabs, a.tiles, sms, a.wk, a.ks)) return B200Q_ERR_CAPACITY;
-  a.slabs_per_cta = (slabs + a.ks - 1) / a.ks;
+  a.slabs_per_cta = ((slabs + a.ks - 1) / a.ks + 1) / 2 * 2;
+  a.pairs = FastDiv(a.slabs_per_cta / 2);
   const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, a.wk, a.ks);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kW4SmemLimit)) != cudaSuccess)
     return B200Q_ERR_CUDA;
-  const int wr = kW4Warps / a.wk;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kW4Threads);
   cfg.dynamicSmemBytes = smem;
@@ -437,7 +496,7 @@ int launch_w4(W4Args a, cudaStream_t s) {
     }
     if (c > 0) room = min(room, c);
   }
-  const int clusters = max(1, min((a.tiles + wr - 1) / wr, room));
+  const int clusters = max(1, min(a.tiles, room));
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * a.ks));
   cudaLaunchKernelEx(&cfg, kern, a);
   return launch_status();
