@@ -1136,7 +1136,7 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
         for r in range(0, m, most):
             call(name, x2.data_ptr() + 2 * r * x2.stride(0), x2.stride(0), _DT[x.dtype], packed.data_ptr(), scales.data_ptr(),
                  extra, bias.data_ptr() if bias is not None else None, out.data_ptr() + 2 * r * n, n, min(most, m - r), n, k,
-                 _stream(x))
+                 qgemm_status(dev).data_ptr(), _stream(x))
     return out
 
 

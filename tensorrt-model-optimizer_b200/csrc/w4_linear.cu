@@ -18,6 +18,8 @@
 // and walks over the row tiles with its part of x resident in shared memory.  Each lane fetches its own operands
 // with cp.async into a ring (kStages x 1 KB a warp, so 96 KB in flight on an SM), which runs on across tiles.
 // Partial sums meet in shared memory, across the cluster through distributed shared memory, in a fixed order.
+#include <math.h>
+
 #include <atomic>
 
 #include "umma.cuh"
@@ -27,11 +29,13 @@ namespace b200q {
 constexpr int kW4Warps = 16, kW4Threads = 32 * kW4Warps;
 constexpr int kW4Rows = 16;                  // weight rows of a tile
 constexpr int kSlab = 128;                   // k elements a warp handles at a time
-#ifndef W4ST
-#define W4ST 3
-#endif
-constexpr int kW4Stages = W4ST;               // of two slabs
-constexpr int kStageBytes = 2048;
+// Slabs of a step and steps of the ring: four slabs make the bookkeeping of a step cheap; with more than 8 rows
+// shared memory is needed for x and the products themselves take longer, so there two have to do.
+template <int NT> struct W4Ring {
+  static constexpr int kSlabs = NT == 1 ? 4 : 2, kStages = 2, kBytes = 1024 * kSlabs;
+};
+inline int w4_ring_bytes(int nt) { return nt == 1 ? W4Ring<1>::kStages * W4Ring<1>::kBytes : W4Ring<2>::kStages * W4Ring<2>::kBytes; }
+constexpr uint32_t kW4WaitCode = 1u << 21;
 
 struct W4Args {
   const void* x;
@@ -45,6 +49,8 @@ struct W4Args {
   int rows, n, k, groups, group_slabs;       // groups a row; slabs a group (groups of 128 and more)
   int slabs_per_cta, tiles, wk, ks;
   FastDiv pairs;                             // slab pairs of a CTA
+  int wide_scales;                           // a lane's scales of a step are one aligned word
+  uint32_t* status;
 };
 
 __device__ __forceinline__ uint32_t w4_pack_f16(float lo, float hi) {
@@ -57,33 +63,49 @@ __device__ __forceinline__ void w4_mma(float* c, uint32_t a0, uint32_t a1, uint3
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same with a zero accumulator
-__device__ __forceinline__ void w4_mma_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+// N words through the read-only path
+template <int N>
+__device__ __forceinline__ void w4_ldg_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else if constexpr (N == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
 }
 template <int N>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+__device__ __forceinline__ void w4_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+// one of the two 16-bit numbers of a word
+template <typename T>
+__device__ __forceinline__ float w4_half_word(uint32_t w, int high) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(high ? w & 0xffff0000u : w << 16);
+  else return __half2float(__ushort_as_half(static_cast<uint16_t>(high ? w >> 16 : w)));
 }
 
-// 8 INT4 codes -> code - 8 as fp16, in the order (1, 5), (0, 4), (3, 7), (2, 6) of the elements
+// 8 INT4 codes as fp16 patterns, one mask for two: a code in the low mantissa bits is the subnormal number
+// code * 2^-24, four bits higher code * 2^-20.  Order (1, 5), (0, 4), (3, 7), (2, 6) of the elements.
 __device__ __forceinline__ void int4x8_to_f16(uint32_t w, uint32_t* h) {
   const uint32_t w8 = w >> 8;
-  uint32_t p0, p1, p2, p3;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p0) : "r"(w), "n"(0x000f000f), "n"(0x64006400));   // (a & b) | c
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p1) : "r"(w), "n"(0x00f000f0), "n"(0x64006400));
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p2) : "r"(w8), "n"(0x000f000f), "n"(0x64006400));
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p3) : "r"(w8), "n"(0x00f000f0), "n"(0x64006400));
-  const uint32_t m1032 = 0xe408e408u, m72 = 0xd480d480u, r16 = 0x2c002c00u;   // -1032, -72, 1/16
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(h[0]) : "r"(p0), "r"(m1032));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(h[1]) : "r"(p1), "r"(r16), "r"(m72));
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(h[2]) : "r"(p2), "r"(m1032));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(h[3]) : "r"(p3), "r"(r16), "r"(m72));
+  h[0] = w & 0x000f000fu;
+  h[1] = w & 0x00f000f0u;
+  h[2] = w8 & 0x000f000fu;
+  h[3] = w8 & 0x00f000f0u;
 }
 // 8 E2M1 codes -> fp16 in element order
 __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t* h) {
@@ -100,6 +122,11 @@ __device__ __forceinline__ uint32_t w4_hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+__device__ __forceinline__ uint32_t w4_hadd2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 __device__ __forceinline__ float rcp_approx(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -112,14 +139,17 @@ enum { kFmtInt4 = 0, kFmtNvfp4 = 1 };
 // so that an instruction's 16 elements always lie in one group of 32 LW (INT4 groups of 32, 64, 128 n).
 template <int FMT, typename T, int NT, int LW>
 __global__ void __launch_bounds__(kW4Threads, 1)
-w4_linear_kernel(const W4Args a) {
+w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   constexpr int kSegs = 4 / LW;                     // groups a slab has (at least)
   constexpr int kRunBytes = 4 * LW;
   constexpr int kPart = kW4Rows * 8 * NT;           // partial sums of a warp
+  constexpr int kStep = W4Ring<NT>::kSlabs, kStages = W4Ring<NT>::kStages, kStageBytes = W4Ring<NT>::kBytes;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint32_t xmax[8 * NT];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
+  __shared__ int not_finite, xbad[8 * NT];          // INT4: x (a row of it) holds an infinity or a NaN
+  if (threadIdx.x < 8 * NT) xbad[threadIdx.x] = not_finite = 0;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
   const int ks = a.ks, wk = a.wk, wr = kW4Warps / wk;
   const int rank = static_cast<int>(cluster_ctarank());
   const int cluster = blockIdx.x / ks, nclusters = gridDim.x / ks;
@@ -127,88 +157,105 @@ w4_linear_kernel(const W4Args a) {
   const int slabs = max(min(a.slabs_per_cta, (a.k + kSlab - 1) / kSlab - slab0), 0);
   const int my_row = warp / wk, my_k = warp % wk;   // which of the CTA's tiles, which part of its slabs
 
-  uint8_t* ring = smem + warp * kW4Stages * kStageBytes;      // [stages][2 slabs][2 rows][32 lanes][16 B]
-  uint8_t* xs = smem + kW4Warps * kW4Stages * kStageBytes; // [slab][i][row][qd] 16 B
-  float* part = reinterpret_cast<float*>(xs + static_cast<int64_t>(a.pairs.d) * 2 * kSlab * 2 * a.rows);   // [warps][8 NT][16], wk > 1
+  uint8_t* ring = smem + warp * kStages * kStageBytes;      // NVFP4: [stages][16 rows][128 B]; INT4: [stages][2 slabs][16 rows][64 B]
+  uint8_t* xs = smem + kW4Warps * kStages * kStageBytes; // [slab][row][i][qd] 16 B
+  float* xsum = reinterpret_cast<float*>(xs + static_cast<int64_t>(a.pairs.d) * 2 * kSlab * 2 * a.rows);   // [slab][group][8 NT], INT4
+  float* part = xsum + (FMT == kFmtInt4 ? static_cast<int>(a.pairs.d) * 2 * kSegs * 8 * NT : 0);           // [warps][8 NT][16], wk > 1
   float* recv = part + (wk > 1 ? kW4Warps * kPart : 0);                           // [ks][wr * 16 * rows / ks], ks > 1
-  const uint32_t ring_addr = smem_u32(ring) + lane * 16;
-
+  __shared__ __align__(8) uint64_t all_bars[kW4Warps * kStages];
+  __shared__ uint32_t abort_flag;
+  uint64_t* bars = all_bars + warp * kStages;
+  if (lane < kStages) mbar_init(&bars[lane], 1);
+  if (threadIdx.x == 0) abort_flag = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
   pdl_prologue();
 
   // tiles of round t: (t * wr + my_row) * nclusters + cluster, so that the last round is spread over the SMs
-  const int npairs = (slabs + 1) / 2;
-  const int mine = npairs > my_k ? (npairs - my_k + wk - 1) / wk : 0;             // slab pairs of this warp in each tile
+  const int nsteps = (slabs + kStep - 1) / kStep;
+  const int mine = nsteps > my_k ? (nsteps - my_k + wk - 1) / wk : 0;             // steps of this warp in each tile
   const int first_tile = my_row * nclusters + cluster, tile_step = wr * nclusters;
   const int rounds = (a.tiles - cluster + tile_step - 1) / tile_step;             // of the CTA
   const int my_tiles = a.tiles > first_tile ? (a.tiles - first_tile + tile_step - 1) / tile_step : 0;
   const int steps = mine * my_tiles;
-  const int64_t row_bytes = a.k / 2;
 
-  // ---- producer: this lane's operands of two slabs of one tile ----
-  // Addresses are kept as pointers that step through a tile's slabs: the arithmetic of an address from
-  // scratch costs as many issue slots as the conversions.
-  const int slab_first = slab0 + 2 * my_k;
-  const int code_step = wk * kSlab;
-  auto row_of = [&](int tile, int r) { return static_cast<int64_t>(min(tile * kW4Rows + gr + 8 * r, a.n - 1)); };
-  const int64_t code_first = slab_first * (kSlab / 2) + qd * kRunBytes;
-  const uint8_t *pc0 = a.codes, *pc1 = a.codes;
-  int p_tile = first_tile, p_i = 0, p_left = steps, p_k = 0;
-  uint32_t p_dst = ring_addr;
-  auto produce = [&]() {
+  // ---- producer: one lane asks for a step's slabs of one tile (rows behind n and elements behind k arrive as zeros) ----
+  const int slab_first = slab0 + kStep * my_k;
+  int p_tile = first_tile, p_i = 0, p_left = steps, p_x = 0;
+  auto produce = [&](uint32_t slot) {
     if (p_left > 0) {
-      if (p_i == 0) {
-        pc0 = a.codes + row_of(p_tile, 0) * row_bytes + code_first;
-        pc1 = a.codes + row_of(p_tile, 1) * row_bytes + code_first;
-        p_k = slab_first * kSlab + qd * 8 * LW;
-        p_tile += tile_step;
-      }
+      if (p_i == 0) p_x = slab_first * (kSlab / 2);
+      if (lane == 0) {
+        uint64_t* bar = reinterpret_cast<uint64_t*>(bars + slot / kStageBytes);
+        mbar_expect_tx(bar, kStageBytes);
+        constexpr int kBox = FMT == kFmtInt4 ? 1 : 2;                              // slabs a copy brings
 #pragma unroll
-      for (int seg = 0; seg < 2 * kSegs; ++seg) {
-        const uint32_t to = p_dst + (seg / kSegs) * 1024 + (seg % kSegs) * kRunBytes;
-        if (p_k + seg * 32 * LW < a.k) {
-          copy_async<kRunBytes>(to, pc0 + seg * 16 * LW);
-          copy_async<kRunBytes>(to + 512, pc1 + seg * 16 * LW);
-        }
+        for (int j = 0; j < kStep; j += kBox)
+          tma_load_2d(ring + slot + 1024 * j, &map, bar, p_x + j * (kSlab / 2), p_tile * kW4Rows);
       }
-      pc0 += code_step;
-      pc1 += code_step;
-      p_k += 2 * code_step;
-      p_i = p_i + 1 == mine ? 0 : p_i + 1;
+      p_x += wk * kStep * (kSlab / 2);
+      if (++p_i == mine) { p_i = 0; p_tile += tile_step; }
       --p_left;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll 1
-  for (int s = 0; s < kW4Stages - 1; ++s) {
-    p_dst = ring_addr + s * kStageBytes;
-    produce();
-  }
+  for (int s = 0; s < kStages; ++s) produce(s * kStageBytes);
 
-  // ---- scales, two slabs ahead of their use ----
-  constexpr int kScales = FMT == kFmtInt4 ? 2 * kSegs : 2;                        // of a row in two slabs
-  constexpr int kScaleSize = FMT == kFmtInt4 ? 2 : 1;
-  using Raw = typename std::conditional<FMT == kFmtInt4, T, uint16_t>::type;      // INT4: a group's scale; NVFP4: two E4M3
-  Raw nxt[2][kScales];
-  const uint8_t *ps0 = nullptr, *ps1 = nullptr;     // the row's scales
+  // ---- scales, one step ahead of their use ----
+  // INT4: 2 kSegs scales of a row in two slabs.  NVFP4: the four E4M3 of the lane's 64 elements.
+  constexpr int kPairs = kStep / 2;
+  constexpr int kScaleWords = kPairs * (FMT == kFmtInt4 ? kSegs : 1);             // of 32 bits
+  uint32_t nxt[2][kScaleWords];
+  const uint8_t* ps[2] = {nullptr, nullptr};        // the rows' scales
   int s_tile = first_tile, s_i = 0, s_left = steps, s_at = 0;
   auto load_scales = [&]() {
     if (s_left > 0) {
       if (s_i == 0) {
-        ps0 = static_cast<const uint8_t*>(a.scales) + row_of(s_tile, 0) * a.groups * kScaleSize;
-        ps1 = static_cast<const uint8_t*>(a.scales) + row_of(s_tile, 1) * a.groups * kScaleSize;
-        s_at = FMT == kFmtInt4 ? slab_first * kSegs : slab_first * (kSlab / 16) + 2 * qd;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          ps[r] = static_cast<const uint8_t*>(a.scales) +
+                  static_cast<int64_t>(min(s_tile * kW4Rows + gr + 8 * r, a.n - 1)) * a.groups * (FMT == kFmtInt4 ? 2 : 1);
+        s_at = FMT == kFmtInt4 ? slab_first * kSegs : slab_first * (kSlab / 16) + 4 * qd;
         s_tile += tile_step;
       }
+      if constexpr (FMT == kFmtInt4) {
 #pragma unroll
-      for (int seg = 0; seg < kScales; ++seg) {
-        int at = FMT == kFmtInt4 ? s_at + seg : s_at + seg * (kSlab / 16);
-        if (FMT == kFmtInt4 && LW == 4 && a.group_slabs > 1) at /= a.group_slabs;
-        at = min(at, a.groups - (FMT == kFmtInt4 ? 1 : 2));                        // behind the end of a row x is zero
-        nxt[0][seg] = __ldg(reinterpret_cast<const Raw*>(ps0 + at * kScaleSize));
-        nxt[1][seg] = __ldg(reinterpret_cast<const Raw*>(ps1 + at * kScaleSize));
+        for (int r = 0; r < 2; ++r) {
+          if (a.wide_scales) {                      // whole steps, aligned
+            w4_ldg_words<kScaleWords>(ps[r] + s_at * 2, nxt[r]);
+          } else {
+#pragma unroll
+            for (int w = 0; w < kScaleWords; ++w) {
+              uint32_t u[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                int at = s_at + 2 * w + h;
+                if (LW == 4) at /= a.group_slabs;
+                at = min(at, a.groups - 1);         // behind the end of a row x is zero
+                u[h] = __ldg(reinterpret_cast<const uint16_t*>(ps[r]) + at);
+              }
+              nxt[r][w] = u[0] | (u[1] << 16);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int w = 0; w < kPairs; ++w) {
+            const int at = s_at + 16 * w;
+            nxt[r][w] = 0;
+            if (a.wide_scales) {
+              if (at < a.groups) nxt[r][w] = __ldg(reinterpret_cast<const uint32_t*>(ps[r] + at));
+            } else {
+              if (at < a.groups) nxt[r][w] = __ldg(reinterpret_cast<const uint16_t*>(ps[r] + at));
+              if (at + 2 < a.groups) nxt[r][w] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(ps[r] + at + 2))) << 16;
+            }
+          }
+        }
       }
-      s_at += FMT == kFmtInt4 ? 2 * wk * kSegs : 2 * wk * (kSlab / 16);
-      s_i = s_i + 1 == mine ? 0 : s_i + 1;
+      s_at += FMT == kFmtInt4 ? kStep * wk * kSegs : kStep * wk * (kSlab / 16);
+      if (++s_i == mine) s_i = 0;
       --s_left;
     }
   };
@@ -222,7 +269,8 @@ w4_linear_kernel(const W4Args a) {
   const T* x = static_cast<const T*>(a.x);
   const int units = a.rows * static_cast<int>(a.pairs.d);
   const int x_i = (lane >> 2) & 3, x_q = lane & 3;
-  const int x_k = slab0 * kSlab + (lane >> 4) * kSlab + ((x_i / LW) * 4 * LW + x_q * LW + x_i % LW) * 8;
+  const int x_k = slab0 * kSlab + (FMT == kFmtInt4 ? (lane >> 4) * kSlab + ((x_i / LW) * 4 * LW + x_q * LW + x_i % LW) * 8
+                                                   : (2 * x_q + (lane >> 4)) * 32 + x_i * 8);
   auto load_x = [&](int u) {
     uint32_t row, pair;
     a.pairs.divmod(u, row, pair);
@@ -254,17 +302,32 @@ w4_linear_kernel(const W4Args a) {
       for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
     }
     uint4 o;
-    if constexpr (FMT == kFmtInt4) {                // (1, 5), (0, 4), (3, 7), (2, 6)
-      o.x = __byte_perm(h[0], h[2], 0x7632);
-      o.y = __byte_perm(h[0], h[2], 0x5410);
+    if constexpr (FMT == kFmtInt4) {
+      // the group's sum, for the 8 in code - 8; elements 0, 4, 2, 6 meet codes that are 16 times too large
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        sum += t.x + t.y;
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if constexpr (LW >= 2) sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      if constexpr (LW == 4) sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      if (!(fabsf(sum) < INFINITY)) not_finite = xbad[row] = 1;
+      if (x_q == 0 && x_i % LW == 0) xsum[(slab * kSegs + x_i / LW) * 8 * NT + row] = sum * -4.76837158203125e-7f;   // -8 * 2^-24
+      o.x = __byte_perm(h[0], h[2], 0x7632);        // (1, 5), (0, 4), (3, 7), (2, 6)
+      o.y = w4_hmul2(__byte_perm(h[0], h[2], 0x5410), 0x2c002c00u);               // / 16
       o.z = __byte_perm(h[1], h[3], 0x7632);
-      o.w = __byte_perm(h[1], h[3], 0x5410);
+      o.w = w4_hmul2(__byte_perm(h[1], h[3], 0x5410), 0x2c002c00u);
     } else {
       o = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    *reinterpret_cast<uint4*>(xs + (((slab * 4 + x_i) * a.rows + static_cast<int>(row)) * 4 + x_q) * 16) = o;
+    // [slab][row][word][q]; odd rows swap words 0, 1 and 2, 3, so that eight lanes of a load hit all banks
+    *reinterpret_cast<uint4*>(xs + (((slab * a.rows + static_cast<int>(row)) * 4 + (x_i ^ (row & 1))) * 4 + x_q) * 16) = o;
   };
   uint4 hold[kHold];
+  if constexpr (!kBf16 && FMT == kFmtInt4) __syncthreads();   // not_finite is 0
 #pragma unroll
   for (int j = 0; j < kHold; ++j) {
     if (warp + j * kW4Warps >= units) break;
@@ -292,15 +355,15 @@ w4_linear_kernel(const W4Args a) {
   if (ks > 1) cluster_barrier(); else __syncthreads();   // the others' shared memory may be written from here on
 
   float back[NT][2];                                // of the columns this thread's sums belong to
-  const float s2 = FMT == kFmtNvfp4 ? __ldg(a.scale2) : 1.f;
+  const float s2 = FMT == kFmtNvfp4 ? __ldg(a.scale2) : 16777216.f;                // 2^24 of the codes as subnormals
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = 8 * n + 2 * qd + j;
-      back[n][j] = s2;
+      back[n][j] = 1.f;
       if constexpr (kBf16)
-        if (row < a.rows) back[n][j] *= __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(xmax[row] >> 7), 28) - 14) << 23);
+        if (row < a.rows) back[n][j] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(xmax[row] >> 7), 28) - 14) << 23);
     }
 
   auto store = [&](int row, int col, float sum) {
@@ -309,14 +372,18 @@ w4_linear_kernel(const W4Args a) {
     static_cast<T*>(a.out)[row * a.out_stride + col] = Elem<T>::from_float(sum);
   };
 
-  uint32_t slot = 0;                                // ring offset of the slab at hand
-  p_dst = ring_addr + (kW4Stages - 1) * kStageBytes;
-  const uint8_t* lane_ring = ring + lane * 16;
+  uint32_t slot = 0, phase = 0;                     // ring offset of the step at hand, parity of its barrier
+  const float* lane_sum = xsum + 2 * qd;
   // x of row 8 n + gr; columns beyond the last row repeat it, their sums are dropped
   const uint8_t* lane_x[NT];
+  int odd[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) lane_x[n] = xs + (min(8 * n + gr, a.rows - 1) * 4 + qd) * 16;
-  const int word_step = 4 * a.rows * 16, slab_step = 4 * word_step;
+  for (int n = 0; n < NT; ++n) {
+    const int row = min(8 * n + gr, a.rows - 1);
+    odd[n] = (row & 1) * 64;
+    lane_x[n] = xs + (kStep * my_k * a.rows + row) * 256 + qd * 16;
+  }
+  const int slab_step = a.rows * 256, pair_step = kStep * wk * slab_step;
 #pragma unroll 1
   for (int round = 0; round < rounds; ++round) {
     const int tile = first_tile + round * tile_step;
@@ -324,32 +391,51 @@ w4_linear_kernel(const W4Args a) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     const int todo = tile < a.tiles ? mine : 0;
+    // signed_too: rows of x that are not finite have the 8 taken off every code instead of off the sum, so that infinity
+    // times (code - 8) keeps its sign; the other rows' arithmetic stays what it is without them
+    auto products = [&](auto signed_too) {
 #pragma unroll 1
-    for (int it = 0; it < todo; ++it) {
-      const uint8_t* xp[NT];
+    for (int it = 0, x_at = 0; it < todo; ++it, x_at += pair_step) {
+      uint32_t cur[2][kScaleWords];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) xp[n] = lane_x[n] + 2 * (my_k + it * wk) * slab_step;
-      Raw cur[2][kScales];
-#pragma unroll
-      for (int seg = 0; seg < kScales; ++seg) { cur[0][seg] = nxt[0][seg]; cur[1][seg] = nxt[1][seg]; }
+      for (int w = 0; w < kScaleWords; ++w) { cur[0][w] = nxt[0][w]; cur[1][w] = nxt[1][w]; }
       load_scales();
-      asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages - 2) : "memory");
+      if (!mbar_wait_bounded(reinterpret_cast<uint64_t*>(bars + slot / kStageBytes), phase, &abort_flag, a.status, kW4WaitCode)) p_left = 0;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {        // behind the end of K x is zero, and the codes whatever they are
-        const uint4 va = *reinterpret_cast<const uint4*>(lane_ring + slot + half * 1024);
-        const uint4 vb = *reinterpret_cast<const uint4*>(lane_ring + slot + half * 1024 + 512);
-        const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+      for (int j4 = 0; j4 < kStep; ++j4) {          // behind the end of K x is zero
+        const int half = j4 & 1;
+        uint32_t wa[4], wb[4];
+        if constexpr (FMT == kFmtNvfp4) {           // 128-byte rows, 16-byte pieces swizzled by the row
+          const uint8_t* p = ring + slot + (j4 / 2) * 2048 + gr * 128 + (((2 * qd + half) ^ gr) << 4);
+          const uint4 va = *reinterpret_cast<const uint4*>(p), vb = *reinterpret_cast<const uint4*>(p + 1024);
+          wa[0] = va.x; wa[1] = va.y; wa[2] = va.z; wa[3] = va.w;
+          wb[0] = vb.x; wb[1] = vb.y; wb[2] = vb.z; wb[3] = vb.w;
+        } else {                                    // 64-byte rows of either slab
+          const uint8_t* p = ring + slot + j4 * 1024 + gr * 64 + qd * kRunBytes;
+#pragma unroll
+          for (int seg = 0; seg < kSegs; ++seg) {
+            w4_words<LW>(p + seg * 4 * kRunBytes, wa + seg * LW);
+            w4_words<LW>(p + seg * 4 * kRunBytes + 512, wb + seg * LW);
+          }
+        }
         uint32_t sc[2][2];
         if constexpr (FMT == kFmtNvfp4) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             uint32_t h;
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(cur[r][half]));
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(cur[r][j4 / 2] >> (16 * half))));
             sc[r][0] = __byte_perm(h, h, 0x1010);
             sc[r][1] = __byte_perm(h, h, 0x3232);
           }
         }
-        float tmp[NT][4];
+        float tmp[NT][4], stmp[NT][4];
+        const uint8_t *xe[NT], *xo[NT];             // words 0, 2 and 1, 3
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint8_t* p = lane_x[n] + x_at + j4 * slab_step;
+          xe[n] = p + odd[n];
+          xo[n] = p + 64 - odd[n];
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t fa[4], fb[4];
@@ -364,16 +450,38 @@ w4_linear_kernel(const W4Args a) {
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint4 b = *reinterpret_cast<const uint4*>(xp[n] + i * word_step);
+            const uint4 b = *reinterpret_cast<const uint4*>((i & 1 ? xo[n] : xe[n]) + (i & 2) * 64);
             if constexpr (FMT == kFmtInt4) {
-              if (i % LW == 0) w4_mma_first(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
-              else w4_mma(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
+              if (i % LW == 0) {                    // from -8 times the sum of the group's x, in the codes' 2^-24
+                const float2 xg = *reinterpret_cast<const float2*>(lane_sum + (kStep * (my_k + it * wk) * kSegs + j4 * kSegs + i / LW) * 8 * NT + 8 * n);
+                tmp[n][0] = tmp[n][2] = xg.x;
+                tmp[n][1] = tmp[n][3] = xg.y;
+              }
+              w4_mma(tmp[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
               w4_mma(tmp[n], fa[2], fb[2], fa[3], fb[3], b.z, b.w);
+              if constexpr (decltype(signed_too)::value) {
+                uint32_t ga[4], gb[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {       // -8 at either scale
+                  ga[j] = w4_hadd2(fa[j], j & 1 ? 0x80808080u : 0x80088008u);
+                  gb[j] = w4_hadd2(fb[j], j & 1 ? 0x80808080u : 0x80088008u);
+                }
+                if (i % LW == 0) stmp[n][0] = stmp[n][1] = stmp[n][2] = stmp[n][3] = 0.f;
+                w4_mma(stmp[n], ga[0], gb[0], ga[1], gb[1], b.x, b.y);
+                w4_mma(stmp[n], ga[2], gb[2], ga[3], gb[3], b.z, b.w);
+              }
               if (i % LW == LW - 1) {
-                const int seg = half * kSegs + i / LW;
-                const float i0 = rcp_approx(Elem<T>::to_float(cur[0][seg])), i1 = rcp_approx(Elem<T>::to_float(cur[1][seg]));
-                acc[n][0] += tmp[n][0] * i0; acc[n][1] += tmp[n][1] * i0;
-                acc[n][2] += tmp[n][2] * i1; acc[n][3] += tmp[n][3] * i1;
+                const int seg = j4 * kSegs + i / LW;
+                const float i0 = rcp_approx(w4_half_word<T>(cur[0][seg / 2], seg & 1)), i1 = rcp_approx(w4_half_word<T>(cur[1][seg / 2], seg & 1));
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  v[j] = tmp[n][j];
+                  if constexpr (decltype(signed_too)::value)
+                    if (xbad[8 * n + 2 * qd + (j & 1)]) v[j] = stmp[n][j];
+                }
+                acc[n][0] += v[0] * i0; acc[n][1] += v[1] * i0;
+                acc[n][2] += v[2] * i1; acc[n][3] += v[3] * i1;
               }
             } else {
               w4_mma(acc[n], fa[0], fb[0], fa[1], fb[1], b.x, b.y);
@@ -381,17 +489,19 @@ w4_linear_kernel(const W4Args a) {
             }
           }
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) xp[n] += slab_step;
       }
-      produce();                                    // into the slot read one step ago
-      p_dst = ring_addr + slot;
-      slot = slot == (kW4Stages - 1) * kStageBytes ? 0 : slot + kStageBytes;
+      __syncwarp();                                 // the slot has been read by every lane
+      produce(slot);
+      slot += kStageBytes;
+      if (slot == kStages * kStageBytes) { slot = 0; phase ^= 1; }
     }
+    };
+    if (FMT == kFmtInt4 && not_finite) products(std::true_type());
+    else products(std::false_type());
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[n][j] *= back[n][j & 1];
+      for (int j = 0; j < 4; ++j) acc[n][j] = acc[n][j] * s2 * back[n][j & 1];
 
     // ---- sums of the K parts, always in the order of the warps and CTAs ----
     const int elems = kW4Rows * a.rows;             // of a tile
@@ -437,40 +547,93 @@ w4_linear_kernel(const W4Args a) {
       if (round + 1 < rounds) cluster_barrier();    // read before the next round's sums arrive
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  grace_after_abort(&abort_flag);
 }
 
-inline size_t w4_smem(int rows, int nt, int slabs, int wk, int ks) {
-  return kW4Warps * kW4Stages * kStageBytes + static_cast<size_t>((slabs + 1) / 2 * 2) * kSlab * 2 * rows +
+// segs: INT4 groups a slab (0: NVFP4)
+inline size_t w4_smem(int rows, int nt, int slabs, int segs, int wk, int ks) {
+  const int step = nt == 1 ? W4Ring<1>::kSlabs : W4Ring<2>::kSlabs;
+  slabs = (slabs + step - 1) / step * step;
+  return kW4Warps * static_cast<size_t>(w4_ring_bytes(nt)) + static_cast<size_t>(slabs) * (kSlab * 2 * rows + 32 * segs * nt) +
          (wk > 1 ? kW4Warps * kW4Rows * 8 * 4 * static_cast<size_t>(nt) : 0) +
          (ks > 1 ? static_cast<size_t>(kW4Warps / wk) * kW4Rows * 4 * rows : 0);
 }
 constexpr size_t kW4SmemLimit = 227 * 1024 - 1024;
 inline int w4_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
-// How K is cut: over the wk warps of a tile and the ks CTAs of a cluster.  x decides the least ks (its part has to fit
-// beside the ring); then wk and after it ks grow until every warp of the GPU has a tile part, while a part keeps two slabs.
-inline bool w4_cut(int rows, int slabs, int tiles, int sms, int& wk, int& ks) {
-  const int nt = w4_nt(rows);
-  for (ks = 1; ks < 8 && w4_smem(rows, nt, (slabs + ks - 1) / ks, 1, ks) > kW4SmemLimit; ks *= 2) {}
-  wk = 1;
-  auto fits = [&](int w, int c) { return w4_smem(rows, nt, (slabs + c - 1) / c, w, c) <= kW4SmemLimit; };
-  if (!fits(1, ks)) return false;
-  auto more = [&] { return static_cast<int64_t>(tiles) * wk * ks * 4 < 3ll * sms * kW4Warps && slabs >= 4 * wk * ks; };
-  while (wk < kW4Warps && more() && fits(2 * wk, ks)) wk *= 2;
-  while (ks < 8 && more() && fits(wk, 2 * ks)) ks *= 2;
-  return true;
+// Clusters of `ks` CTAs that run at a time when each fills its SM: a cluster's SMs are of one GPC, so large
+// clusters leave some SMs without work (148 SMs: 74, 33 and 15 clusters of 2, 4 and 8).
+inline int w4_clusters(const void* kern, int ks, int sms) {
+  if (ks == 1) return sms;
+  static std::atomic<int> cached[3];                // clusters of 2, 4, 8
+  std::atomic<int>& slot = cached[ks == 2 ? 0 : ks == 4 ? 1 : 2];
+  int c = slot;
+  if (c == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(sms / ks * ks));
+    cfg.blockDim = dim3(kW4Threads);
+    cfg.dynamicSmemBytes = kW4SmemLimit;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ks);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) != cudaSuccess || c <= 0) {
+      cudaGetLastError();
+      c = sms / ks;
+    }
+    slot = c;
+  }
+  return c;
+}
+
+// How K is cut over the wk warps of a tile and the ks CTAs of a cluster: the least of an estimate in steps of a
+// fully loaded SM.  A round takes a warp's steps in it; one that leaves warps idle is shorter, but not below what a
+// warp needs by itself (0.6); and each round that joins sums pays for its barriers.
+inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, const void* kern, int& wk, int& ks, int& clusters) {
+  const int nt = w4_nt(rows), step = nt == 1 ? W4Ring<1>::kSlabs : W4Ring<2>::kSlabs;
+  double best = 1e30;
+  for (int c = 1; c <= 8; c *= 2) {
+    const int part = (slabs + c - 1) / c, steps = (part + step - 1) / step;
+    if (c > 1 && part * c / 2 > slabs) break;       // no slab left for the last CTAs
+    for (int w = 1; w <= kW4Warps && (w == 1 || w <= steps); w *= 2) {
+      if (w4_smem(rows, nt, part, segs, w, c) > kW4SmemLimit) continue;
+      const int held = w4_clusters(kern, c, sms);
+      const double load = static_cast<double>(tiles) * w / (static_cast<double>(held) * kW4Warps);
+      const double whole = floor(load), rest = load - whole;
+      const double rounds = ceil(load), mine = (steps + w - 1) / w;
+      const double cost = mine * (whole + (rest > 0 ? (rest > 0.6 ? rest : 0.6) : 0)) + rounds * ((w > 1 ? 0.15 : 0) + (c > 1 ? 0.4 : 0)) +
+                          (c > 1 ? 0.3 : 0);
+      if (cost < best) { best = cost; wk = w; ks = c; clusters = held; }
+    }
+  }
+  return best < 1e30;
 }
 
 template <int FMT, typename T, int NT, int LW>
 int launch_w4(W4Args a, cudaStream_t s) {
   auto kern = w4_linear_kernel<FMT, T, NT, LW>;
   const int slabs = (a.k + kSlab - 1) / kSlab, sms = sm_count_cached();
-  if (!w4_cut(a.rows, slabs, a.tiles, sms, a.wk, a.ks)) return B200Q_ERR_CAPACITY;
-  a.slabs_per_cta = ((slabs + a.ks - 1) / a.ks + 1) / 2 * 2;
-  a.pairs = FastDiv(a.slabs_per_cta / 2);
-  const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, a.wk, a.ks);
+  constexpr int kStep = W4Ring<NT>::kSlabs;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kW4SmemLimit)) != cudaSuccess)
+    return B200Q_ERR_CUDA;
+  int room = 0;                                     // after the attribute above: the occupancy depends on it
+  if (!w4_cut(a.rows, slabs, FMT == kFmtInt4 ? 4 / LW : 0, a.tiles, sms, reinterpret_cast<const void*>(kern), a.wk, a.ks, room))
+    return B200Q_ERR_CAPACITY;
+  a.slabs_per_cta = ((slabs + a.ks - 1) / a.ks + kStep - 1) / kStep * kStep;
+  a.pairs = FastDiv(a.slabs_per_cta / 2);
+  const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, FMT == kFmtInt4 ? 4 / LW : 0, a.wk, a.ks);
+  const int unit = FMT == kFmtInt4 ? W4Ring<NT>::kSlabs * 4 / LW : 4, bytes = FMT == kFmtInt4 ? 2 : 1;   // scales a lane takes at a time
+  a.wide_scales = (FMT == kFmtNvfp4 || LW < 4 || a.group_slabs == 1) && a.groups % unit == 0 &&
+                  reinterpret_cast<uintptr_t>(a.scales) % min(unit * bytes, 16) == 0;
+  CUtensorMap map;
+  const EncodeTiledFn encode = encode_tiled_fn();
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.k) / 2, static_cast<cuuint64_t>(a.n)}, strides[1] = {static_cast<cuuint64_t>(a.k) / 2};
+  const cuuint32_t box[2] = {FMT == kFmtInt4 ? 64u : 128u, kW4Rows}, ones[2] = {1, 1};
+  if (!encode || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.codes), dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, FMT == kFmtInt4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return B200Q_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kW4Threads);
@@ -484,21 +647,9 @@ int launch_w4(W4Args a, cudaStream_t s) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  int room = sms / a.ks;                            // clusters the GPU holds at a time (they need SMs of one GPC)
-  if (a.ks > 2) {
-    static std::atomic<int> cached[2];              // clusters of 4, of 8; every block has an SM to itself
-    int c = cached[a.ks == 4 ? 0 : 1];
-    if (c == 0) {
-      int got = 0;
-      cfg.gridDim = dim3(static_cast<unsigned>(room * a.ks));
-      if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) == cudaSuccess && got > 0)
-        cached[a.ks == 4 ? 0 : 1] = c = got;
-    }
-    if (c > 0) room = min(room, c);
-  }
   const int clusters = max(1, min(a.tiles, room));
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * a.ks));
-  cudaLaunchKernelEx(&cfg, kern, a);
+  cudaLaunchKernelEx(&cfg, kern, map, a);
   return launch_status();
 }
 
@@ -526,8 +677,9 @@ inline int w4_check(const void* x, int64_t x_stride, int dtype, const uint8_t* c
 }
 
 inline W4Args w4_args(const void* x, int64_t x_stride, const uint8_t* codes, const void* scales, const float* scale2,
-                      const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, int block) {
+                      const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, int block, uint32_t* status) {
   W4Args a{};
+  a.status = status;
   a.x = x; a.x_stride = x_stride; a.codes = codes; a.scales = scales; a.scale2 = scale2; a.bias = bias;
   a.out = out; a.out_stride = out_stride;
   a.rows = rows; a.n = static_cast<int>(n); a.k = static_cast<int>(k);
@@ -545,16 +697,17 @@ extern "C" int b200q_w4_linear_max_rows(int64_t k) {
   if (k <= 0 || k % 32 || k > (1 << 24)) return 0;
   const int slabs = static_cast<int>((k + kSlab - 1) / kSlab);
   for (int rows = 32; rows > 0; --rows)
-    if (w4_smem(rows, w4_nt(rows), (slabs + 7) / 8, 1, 8) <= kW4SmemLimit) return rows;
+    if (w4_smem(rows, w4_nt(rows), (slabs + 7) / 8, 4, 1, 8) <= kW4SmemLimit) return rows;
   return 0;
 }
 
 extern "C" int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const void* scales, int block,
-                                 const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, void* stream) {
+                                 const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, uint32_t* status_io, void* stream) {
+  B200Q_REQUIRE_PTR(status_io);
   if (const int r = w4_check(x, x_stride, dtype, codes, scales, out, out_stride, rows, n, k)) return r;
   if (block <= 0 || k % block) return B200Q_ERR_SHAPE;
   if (block != 32 && block != 64 && block % kSlab) return B200Q_ERR_UNSUPPORTED;
-  const W4Args a = w4_args(x, x_stride, codes, scales, nullptr, bias, out, out_stride, rows, n, k, block);
+  const W4Args a = w4_args(x, x_stride, codes, scales, nullptr, bias, out, out_stride, rows, n, k, block, status_io);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (block == 32) return dispatch_w4<kFmtInt4, 1>(a, dtype, s);
   if (block == 64) return dispatch_w4<kFmtInt4, 2>(a, dtype, s);
@@ -563,9 +716,10 @@ extern "C" int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, con
 
 extern "C" int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales,
                                   const float* scale2, const void* bias, void* out, int64_t out_stride, int rows, int64_t n,
-                                  int64_t k, void* stream) {
+                                  int64_t k, uint32_t* status_io, void* stream) {
+  B200Q_REQUIRE_PTR(status_io);
   if (const int r = w4_check(x, x_stride, dtype, codes, scales, out, out_stride, rows, n, k)) return r;
   B200Q_REQUIRE_PTR(scale2);
-  const W4Args a = w4_args(x, x_stride, codes, scales, scale2, bias, out, out_stride, rows, n, k, 16);
+  const W4Args a = w4_args(x, x_stride, codes, scales, scale2, bias, out, out_stride, rows, n, k, 16, status_io);
   return dispatch_w4<kFmtNvfp4, 4>(a, dtype, static_cast<cudaStream_t>(stream));
 }

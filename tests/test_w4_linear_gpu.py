@@ -123,6 +123,8 @@ def test_bf16_rows_of_any_magnitude(scale):
     x[1] *= 2.0 ** -60 if scale > 1 else 1                 # rows are scaled one by one
     assert torch.isfinite(x).all()
     _close(ops.nvfp4_linear(x, packed, scales, s2), x, w)
+    packed, scales, w = _int4(40, 1024, 128, torch.bfloat16, seed=2)
+    _close(ops.int4_linear(x, packed, scales, 128), x, w)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
