@@ -4,14 +4,15 @@
 // over the tokens j that query t of its request sees (its own position and everything before it).
 //
 // Work.  A segment is one kv head of one request and one tile of 8 NT query rows (query tokens x the heads
-// that share the kv head); its cache tokens are cut into tiles of 64.  All tiles of all segments form one line
+// that share the kv head); its cache tokens are cut into tiles of 128.  All tiles of all segments form one line
 // that is dealt out to the CTAs in equal contiguous shares, so ragged lengths balance without the host knowing
 // a length.  A segment that lies inside one share is finished there; pieces of the others go to a workspace as
 // (max, sum, unnormalised output) and kv_merge_kernel joins them in a fixed order.
 //
-// Inside a CTA the four warps take 16 tokens of each tile.  A warp's codes and scales come by four bulk copies
-// per 16 tokens (1 KB + 128 B each for K and V at D = 128) into a ring of its own, kStages deep, with the page ids
-// read ahead; there is no block-wide barrier before the end of a segment.
+// Inside a CTA the four warps take 32 tokens of each tile.  A warp's codes and scales come by four bulk copies
+// per 32 tokens (2 KB + 256 B each for K and V at D = 128; per 16 tokens where pages are not multiples of 32) into a
+// ring of its own, two steps deep, with the page ids read ahead; there is no block-wide barrier before the end of a
+// segment.
 //
 // Mathematics.  S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: cache tokens (or head dimensions) fill the 16
 // rows, the query rows the 8 columns, so a group of up to eight heads wastes nothing.  E2M1 times E4M3 has at
@@ -28,8 +29,9 @@ namespace b200q {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kChunk = 16;                          // tokens a warp handles at a time
-constexpr int kTile = kChunk * kAttnWarps;          // tokens of a tile
+constexpr int kChunk = 16;                          // tokens of a matrix product
+constexpr int kStep = 2 * kChunk;                   // tokens a warp handles at a time
+constexpr int kTile = kStep * kAttnWarps;           // tokens of a tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kAttnWaitCode = 1u << 20;
 
@@ -48,6 +50,7 @@ struct AttnArgs {
   float2* part_ml;                                  // [ctas, 2, rows]
   int4* desc;                                       // [ctas]: request, head, row tile, pieces
   uint32_t* status;
+  FastDiv chunks_per_page, group_div;
   int width, requests, tokens, heads, group, page, pages, zero_tail;
   float scale;
 };
@@ -97,7 +100,7 @@ __device__ __forceinline__ void next_segment(const AttnArgs& a, Cursor& c) {
 
 // tokens that query row `row` (query token * group + head) of a request sees
 __device__ __forceinline__ int row_limit(const AttnArgs& a, const Request& r, int row) {
-  const int i = min(row / a.group, r.nq - 1);
+  const int i = min(static_cast<int>(a.group_div.div(row)), r.nq - 1);
   return min(max(r.len - r.nq + i + 1, 0), r.len);
 }
 
@@ -161,9 +164,9 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t* w) {
 template <int D, int NT>
 struct AttnShape {
   static constexpr int kRT = 8 * NT;
-  static constexpr int kCodeBytes = kChunk * D / 2, kScaleBytes = kChunk * D / 16;
+  static constexpr int kCodeBytes = kStep * D / 2, kScaleBytes = kStep * D / 16;
   static constexpr int kSlot = 2 * (kCodeBytes + kScaleBytes);
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 2;
   static constexpr int kRing = kAttnWarps * kStages * kSlot;
   static constexpr int kMerge = kAttnWarps * kRT * D * 4;
   static constexpr int kSmem = kRing + kMerge;
@@ -182,11 +185,11 @@ kv_attention_kernel(const AttnArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kAttnWarps * ST];
   __shared__ int64_t scan_sums[kAttnWarps];
-  __shared__ Cursor start;
+  __shared__ Cursor cc, pcs[kAttnWarps];            // where the CTA's products and each warp's copies are: read between segments only
   __shared__ uint32_t abort_flag;
   __shared__ float2 merge_ml[kAttnWarps][RT];
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
   if (threadIdx.x < kAttnWarps * ST) mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -233,52 +236,83 @@ kv_attention_kernel(const AttnArgs a) {
     const int64_t seg = in / c.r.nkt;
     c.rt = static_cast<int>(seg % c.r.nrt);
     c.h = static_cast<int>(seg / c.r.nrt);
-    start = c;
+    cc = c;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) pcs[w] = c;
   }
   __syncthreads();
 
-  // ---- the warp's producer: bulk copies of 16 tokens into a ring of its own ----
+  // ---- the warp's producer: bulk copies of 32 tokens into a ring of its own ----
   uint8_t* ring = smem + warp * ST * S::kSlot;
   uint64_t* bar = bars + warp * ST;
-  Cursor pc = start;
+  const bool wide = a.page % kStep == 0;            // the 32 tokens of a step lie in one page
+  Cursor& pc = pcs[warp];
+  int p_kt = pc.kt, p_nkt = pc.r.nkt, p_head = pc.h;
+  const int* p_row = a.table + pc.b * a.table_stride;
   int64_t p_left = t1 - t0;
-  uint32_t live = 0, phase = 0;                     // bit s: slot s holds (or awaits) a chunk; parity of its barrier
-  int p_slot = 0, p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1), p_id = -1;
-  auto page_of = [&]() {                            // page id of the producer's chunk, -1 where there is nothing to read
-    const int tok = pc.kt * kTile + warp * kChunk;
-    if (p_left <= 0 || tok >= p_limit) return -1;
-    const int id = a.table[pc.b * a.table_stride + tok / a.page];
-    return id < a.pages ? id : -1;
+  uint32_t live = 0, phase = 0;                     // bits 2s, 2s + 1: the halves of slot s that hold (or await) tokens; parities
+  int p_slot = 0, p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
+  int p_id[2], p_in[2];                             // page ids of the step's halves (-1: nothing to read), tokens into the page
+  auto look_up = [&]() {
+    p_id[0] = p_id[1] = -1;
+    const int tok = p_kt * kTile + warp * kStep;
+    if (p_left <= 0 || tok >= p_limit) return;
+    uint32_t col, in;
+    a.chunks_per_page.divmod(tok / kChunk, col, in);
+    int id = __ldg(p_row + col);
+    p_id[0] = id < a.pages ? id : -1;
+    p_in[0] = in * kChunk;
+    if (tok + kChunk < p_limit) {
+      p_in[1] = p_in[0] + kChunk;
+      if (!wide && ++in == a.chunks_per_page.d) {   // the second half begins the next page
+        id = __ldg(p_row + col + 1);
+        p_in[1] = 0;
+      }
+      p_id[1] = id < a.pages ? id : -1;
+    }
   };
-  p_id = page_of();
+  look_up();
   auto produce = [&]() {
-    const bool ok = p_id >= 0;
-    if (ok && lane == 0) {
-      const int tok = pc.kt * kTile + warp * kChunk;
-      const int64_t row = (static_cast<int64_t>(p_id) * a.heads + pc.h) * a.page + tok % a.page;
+    const bool ok0 = p_id[0] >= 0, ok1 = p_id[1] >= 0;
+    if (lane == 0 && (ok0 || ok1)) {
       uint8_t* dst = ring + p_slot * S::kSlot;
       uint64_t* b = bar + p_slot;
-      mbar_expect_tx(b, S::kSlot);
-      bulk_load(dst, a.k_codes + row * (D / 2), S::kCodeBytes, b);
-      bulk_load(dst + S::kCodeBytes, a.v_codes + row * (D / 2), S::kCodeBytes, b);
-      bulk_load(dst + 2 * S::kCodeBytes, a.k_scales + row * (D / 16), S::kScaleBytes, b);
-      bulk_load(dst + 2 * S::kCodeBytes + S::kScaleBytes, a.v_scales + row * (D / 16), S::kScaleBytes, b);
+      mbar_expect_tx(b, ok0 && ok1 ? S::kSlot : S::kSlot / 2);
+      auto copy = [&](int half, int id, int in, int share) {                       // 1 / share of a slot
+        const int64_t row = (static_cast<int64_t>(id) * a.heads + p_head) * a.page + in;
+        uint8_t* c = dst + half * (S::kCodeBytes / 2);
+        uint8_t* s = dst + 2 * S::kCodeBytes + half * (S::kScaleBytes / 2);
+        bulk_load(c, a.k_codes + row * (D / 2), S::kCodeBytes / share, b);
+        bulk_load(c + S::kCodeBytes, a.v_codes + row * (D / 2), S::kCodeBytes / share, b);
+        bulk_load(s, a.k_scales + row * (D / 16), S::kScaleBytes / share, b);
+        bulk_load(s + S::kScaleBytes, a.v_scales + row * (D / 16), S::kScaleBytes / share, b);
+      };
+      if (wide && ok1) {
+        copy(0, p_id[0], p_in[0], 1);
+      } else {
+        if (ok0) copy(0, p_id[0], p_in[0], 2);
+        if (ok1) copy(1, p_id[1], p_in[1], 2);
+      }
     }
-    live = (live & ~(1u << p_slot)) | (static_cast<uint32_t>(ok) << p_slot);
+    live = (live & ~(3u << (2 * p_slot))) | ((ok0 ? 1u : 0u) | (ok1 ? 2u : 0u)) << (2 * p_slot);
     p_slot = p_slot + 1 == ST ? 0 : p_slot + 1;
     if (--p_left > 0) {
-      if (++pc.kt == pc.r.nkt) {
-        next_segment<RT>(a, pc);
+      if (++p_kt == p_nkt) {
+        if (lane == 0) next_segment<RT>(a, pc);
+        __syncwarp();
+        p_kt = 0;
+        p_nkt = pc.r.nkt;
+        p_head = pc.h;
+        p_row = a.table + pc.b * a.table_stride;
         p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
       }
     }
-    p_id = page_of();
+    look_up();
   };
 #pragma unroll 1
   for (int s = 0; s < ST; ++s) produce();
 
   const float qk = a.scale * kLog2e * __ldg(a.k_scale2), v2 = __ldg(a.v_scale2);
-  Cursor cc = start;
   int64_t left = t1 - t0;
   int slot = 0;
   int4 my_desc = make_int4(0, 0, 0, 0);
@@ -299,7 +333,9 @@ kv_attention_kernel(const AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) qf[n][i] = 0;
       if (8 * n + gr < rows) {
-        const int tok = row / a.group, hd = cc.h * a.group + row % a.group;
+        uint32_t tok, hd;
+        a.group_div.divmod(row, tok, hd);
+        hd += cc.h * a.group;
         const T* src = static_cast<const T*>(a.q) + (cc.r.q0 + tok) * a.q_token_stride + hd * a.q_head_stride + qd * (D / 4);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -330,41 +366,46 @@ kv_attention_kernel(const AttnArgs a) {
       }
     }
     float o[NT][D / 16][4];
-    float m[NT][2], l[NT][2];
+    float m[NT][2], ms[NT][2], l[NT][2];            // ms: m, or 0 while nothing has been seen
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
+      ms[n][0] = ms[n][1] = 0.f;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
     }
 
+    // row gr of the 16 x 8 product is token gr ^ bit 1 of gr: both operands' shared-memory reads then spread
+    const int tg = gr ^ ((gr >> 1) & 1);
+    // the tokens of V's operand: rows 2 qd and 2 qd + 1, and the same + 8
+    const int ta = (2 * qd) ^ (qd & 1), tb = ta ^ 1;
+
 #pragma unroll 1
     for (int kt = cc.kt; kt < kt_end; ++kt) {
-      const bool here = (live >> slot) & 1u;
-      const bool landed = here && __all_sync(0xffffffffu, mbar_wait_bounded(bar + slot, (phase >> slot) & 1u, &abort_flag,
-                                                                            a.status, kAttnWaitCode));
-      if (here && !landed) p_left = 0;              // gave up: nothing more is asked for
+      const uint32_t here = (live >> (2 * slot)) & 3u;
+      const bool landed = here != 0 && __all_sync(0xffffffffu, mbar_wait_bounded(bar + slot, (phase >> slot) & 1u, &abort_flag,
+                                                                                 a.status, kAttnWaitCode));
+      if (here != 0 && !landed) p_left = 0;         // gave up: nothing more is asked for
       if (landed) {
         const uint8_t* kc = ring + slot * S::kSlot;
         const uint8_t* vc = kc + S::kCodeBytes;
         const uint8_t* ks = kc + 2 * S::kCodeBytes;
         const uint8_t* vs = ks + S::kScaleBytes;
-        const int tok0 = kt * kTile + warp * kChunk;
-        // row gr of the 16 x 8 product is token gr ^ bit 1 of gr: both operands' shared-memory reads then spread
-        const int tg = gr ^ ((gr >> 1) & 1);
-        // ---- scores ----
-        float s[NT][4];
+        const int tok0 = kt * kTile + warp * kStep;
+        // ---- scores of 32 tokens ----
+        float s[2][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        {
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[c][n][0] = s[c][n][1] = s[c][n][2] = s[c][n][3] = 0.f;
           uint32_t w[2][KW];
-          lds_words<4 * KW>(kc + tg * (D / 2) + qd * (D / 8), w[0]);
-          lds_words<4 * KW>(kc + (tg + 8) * (D / 2) + qd * (D / 8), w[1]);
+          lds_words<4 * KW>(kc + (c * kChunk + tg) * (D / 2) + qd * (D / 8), w[0]);
+          lds_words<4 * KW>(kc + (c * kChunk + tg + 8) * (D / 2) + qd * (D / 8), w[1]);
           uint32_t sc[2][KB];                       // block scales, each twice
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint8_t* p = ks + (tg + 8 * r) * (D / 16) + qd * KB;
+            const uint8_t* p = ks + (c * kChunk + tg + 8 * r) * (D / 16) + qd * KB;
 #pragma unroll
             for (int i = 0; i < KB; i += 2) {
               const uint32_t two = KB == 1 ? *p : *reinterpret_cast<const uint16_t*>(p + i);
@@ -382,24 +423,29 @@ kv_attention_kernel(const AttnArgs a) {
             for (int j = 0; j < 4; ++j) { x[j] = hmul2(x[j], sc[0][i / 2]); y[j] = hmul2(y[j], sc[1][i / 2]); }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma_f16(s[n], x[0], y[0], x[1], y[1], qf[n][4 * i], qf[n][4 * i + 1]);
-              mma_f16(s[n], x[2], y[2], x[3], y[3], qf[n][4 * i + 2], qf[n][4 * i + 3]);
+              mma_f16(s[c][n], x[0], y[0], x[1], y[1], qf[n][4 * i], qf[n][4 * i + 1]);
+              mma_f16(s[c][n], x[2], y[2], x[3], y[3], qf[n][4 * i + 2], qf[n][4 * i + 3]);
             }
           }
         }
         // ---- softmax, base 2 ----
-        const bool masked = tok0 + kChunk > lim_lo;
+        const bool masked = tok0 + kStep > lim_lo || here != 3u;
         bool grow = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][j] *= qs[n][j & 1];
-          if (masked) {
+          for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (tok0 + tg + 8 * (j >> 1) >= lim[n][j & 1]) s[n][j] = -INFINITY;
+            for (int j = 0; j < 4; ++j) s[c][n][j] *= qs[n][j & 1];
+            if (masked) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (tok0 + c * kChunk + tg + 8 * (j >> 1) >= lim[n][j & 1] || !(here >> c & 1u)) s[c][n][j] = -INFINITY;
+            }
           }
-          grow |= fmaxf(s[n][0], s[n][2]) > m[n][0] + 8.f || fmaxf(s[n][1], s[n][3]) > m[n][1] + 8.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            grow |= fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])) > m[n][j] + 8.f;
         }
         // the reference maximum follows only when a score passes it by 2^8 (P stays within fp16): rarely
         if (__any_sync(0xffffffffu, grow)) {
@@ -407,119 +453,129 @@ kv_attention_kernel(const AttnArgs a) {
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float t = fmaxf(s[n][j], s[n][j + 2]);
+              float t = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
               t = fmaxf(t, m[n][j]);
               const float f = m[n][j] == t ? 1.f : exp2_fast(m[n][j] - t);
               m[n][j] = t;
+              ms[n][j] = t == -INFINITY ? 0.f : t;
               l[n][j] *= f;
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) { o[n][i][j] *= f; o[n][i][j + 2] *= f; }
             }
           }
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[2][NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-          const float p0 = exp2_fast(s[n][0] - m0), p1 = exp2_fast(s[n][1] - m1);
-          const float p2 = exp2_fast(s[n][2] - m0), p3 = exp2_fast(s[n][3] - m1);
-          l[n][0] += p0 + p2;
-          l[n][1] += p1 + p3;
-          pb[n][0] = transpose8x8(pack_f16(p0, p1));
-          pb[n][1] = transpose8x8(pack_f16(p2, p3));
-        }
-        // ---- output: tokens 2qd, 2qd + 1 (one swapped pair of rows) and the same + 8 ----
-        const int ta = (2 * qd) ^ (qd & 1), tb = ta ^ 1;
-        uint32_t wa[2][VW], wb[2][VW];
-        uint32_t sb[2][VB];                         // scale bytes of a token pair
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          lds_words<4 * VW>(vc + (ta + 8 * r) * (D / 2) + gr * (D / 16), wa[r]);
-          lds_words<4 * VW>(vc + (tb + 8 * r) * (D / 2) + gr * (D / 16), wb[r]);
+          for (int n = 0; n < NT; ++n) {
+            const float p0 = exp2_fast(s[c][n][0] - ms[n][0]), p1 = exp2_fast(s[c][n][1] - ms[n][1]);
+            const float p2 = exp2_fast(s[c][n][2] - ms[n][0]), p3 = exp2_fast(s[c][n][3] - ms[n][1]);
+            l[n][0] += p0 + p2;
+            l[n][1] += p1 + p3;
+            pb[c][n][0] = transpose8x8(pack_f16(p0, p1));
+            pb[c][n][1] = transpose8x8(pack_f16(p2, p3));
+          }
+        // ---- output: tokens ta, tb and the same + 8 of either half ----
+        uint32_t sb[2][2][VB];                      // scale bytes of a token pair
 #pragma unroll
-          for (int i = 0; i < VB; ++i) {
-            const int blk = D >= 128 ? gr * VB + i : gr >> 1;
-            uint32_t x = vs[(ta + 8 * r) * (D / 16) + blk], y = vs[(tb + 8 * r) * (D / 16) + blk];
-            if (masked) {                           // behind the last token anything may stand: 0 * NaN is NaN
-              if (tok0 + ta + 8 * r >= lim_hi) x = 0;
-              if (tok0 + tb + 8 * r >= lim_hi) y = 0;
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < VB; ++i) {
+              const int blk = D >= 128 ? gr * VB + i : gr >> 1, t = c * kChunk + 8 * r;
+              sb[c][r][i] = vs[(ta + t) * (D / 16) + blk] | (vs[(tb + t) * (D / 16) + blk] << 8);
             }
-            sb[r][i] = x | (y << 8);
-          }
-        }
-        auto v_frag = [&](int j, const uint32_t (*sc)[VB], uint32_t* f) {   // operand of dimensions 2j, 2j + 1 of the run: slow form
-          const int w = j / 4, by = 8 * (j % 4);
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t lo = (wa[r][w] & 0x0f0f0f0fu) | ((wb[r][w] << 4) & 0xf0f0f0f0u);
-            const uint32_t hi = ((wa[r][w] >> 4) & 0x0f0f0f0fu) | (wb[r][w] & 0xf0f0f0f0u);
-            uint32_t x[4], y[4];
-            cvt_e2m1x8(lo >> by, x);
-            cvt_e2m1x8(hi >> by, y);
-            const uint32_t sh = cvt_e4m3x2(sc[r][w / 2]);
-            f[2 * r] = hmul2(x[0], sh);
-            f[2 * r + 1] = hmul2(y[0], sh);
-          }
-        };
         bool nan_v = false;
-        if (masked && lim_lo < lim_hi) {            // some rows see tokens that others do not
+        if (masked) {                               // behind the last token anything may stand: 0 * NaN is NaN
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < VB; ++i) nan_v |= (sb[r][i] & 0x7fu) == 0x7fu || (sb[r][i] & 0x7f00u) == 0x7f00u;
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int i = 0; i < VB; ++i) {
+                const int t = tok0 + c * kChunk + 8 * r;
+                const bool on = here >> c & 1u;
+                sb[c][r][i] &= (on && t + ta < lim_hi ? 0xffu : 0u) | (on && t + tb < lim_hi ? 0xff00u : 0u);
+                // some rows see tokens that others do not
+                nan_v |= lim_lo < lim_hi && ((sb[c][r][i] & 0x7fu) == 0x7fu || (sb[c][r][i] & 0x7f00u) == 0x7f00u);
+              }
         }
-        if (!__any_sync(0xffffffffu, nan_v)) {
-          uint32_t sh[2][VB];
+        if (!masked || !__any_sync(0xffffffffu, nan_v)) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int i = 0; i < VB; ++i) sh[r][i] = cvt_e4m3x2(sb[r][i]);
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            uint32_t x[2][4], y[2][4];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t wa[2][VW], wb[2][VW], sh[2][VB];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              cvt_e2m1x8((wa[r][w] & 0x0f0f0f0fu) | ((wb[r][w] << 4) & 0xf0f0f0f0u), x[r]);
-              cvt_e2m1x8(((wa[r][w] >> 4) & 0x0f0f0f0fu) | (wb[r][w] & 0xf0f0f0f0u), y[r]);
+              lds_words<4 * VW>(vc + (c * kChunk + ta + 8 * r) * (D / 2) + gr * (D / 16), wa[r]);
+              lds_words<4 * VW>(vc + (c * kChunk + tb + 8 * r) * (D / 2) + gr * (D / 16), wb[r]);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) { x[r][j] = hmul2(x[r][j], sh[r][w / 2]); y[r][j] = hmul2(y[r][j], sh[r][w / 2]); }
+              for (int i = 0; i < VB; ++i) sh[r][i] = cvt_e4m3x2(sb[c][r][i]);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int w = 0; w < VW; ++w) {
+              uint32_t x[2][4], y[2][4];
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(o[n][4 * w + j], x[0][j], y[0][j], x[1][j], y[1][j], pb[n][0], pb[n][1]);
+              for (int r = 0; r < 2; ++r) {
+                cvt_e2m1x8((wa[r][w] & 0x0f0f0f0fu) | ((wb[r][w] << 4) & 0xf0f0f0f0u), x[r]);
+                cvt_e2m1x8(((wa[r][w] >> 4) & 0x0f0f0f0fu) | (wb[r][w] & 0xf0f0f0f0u), y[r]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { x[r][j] = hmul2(x[r][j], sh[r][w / 2]); y[r][j] = hmul2(y[r][j], sh[r][w / 2]); }
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_f16(o[n][4 * w + j], x[0][j], y[0][j], x[1][j], y[1][j], pb[c][n][0], pb[c][n][1]);
+            }
           }
         } else {
           // A NaN value that only some rows may see: each row's product on its own, with what it does not see
           // zeroed, and only that row's column kept.
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t wa[2][VW], wb[2][VW];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              lds_words<4 * VW>(vc + (c * kChunk + ta + 8 * r) * (D / 2) + gr * (D / 16), wa[r]);
+              lds_words<4 * VW>(vc + (c * kChunk + tb + 8 * r) * (D / 2) + gr * (D / 16), wb[r]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll 1
-            for (int col = 0; col < 8; ++col) {
-              const int see = row_limit(a, cc.r, row0 + 8 * n + col);
-              uint32_t sc[2][VB];
+              for (int col = 0; col < 8; ++col) {
+                const int see = row_limit(a, cc.r, row0 + 8 * n + col) - tok0 - c * kChunk;
 #pragma unroll
-              for (int r = 0; r < 2; ++r)
+                for (int w = 0; w < VW; ++w) {
 #pragma unroll
-                for (int i = 0; i < VB; ++i)
-                  sc[r][i] = sb[r][i] & ((tok0 + ta + 8 * r < see ? 0xffu : 0u) | (tok0 + tb + 8 * r < see ? 0xff00u : 0u));
+                  for (int j = 0; j < 4; ++j) {
+                    uint32_t f[4];
 #pragma unroll
-              for (int j = 0; j < D / 16; ++j) {
-                uint32_t f[4];
-                v_frag(j, sc, f);
-                float t[4] = {o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]};
-                mma_f16(t, f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
-                if (col == 2 * qd) { o[n][j][0] = t[0]; o[n][j][2] = t[2]; }
-                if (col == 2 * qd + 1) { o[n][j][1] = t[1]; o[n][j][3] = t[3]; }
+                    for (int r = 0; r < 2; ++r) {
+                      uint32_t x[4], y[4];
+                      cvt_e2m1x8((wa[r][w] & 0x0f0f0f0fu) | ((wb[r][w] << 4) & 0xf0f0f0f0u), x);
+                      cvt_e2m1x8(((wa[r][w] >> 4) & 0x0f0f0f0fu) | (wb[r][w] & 0xf0f0f0f0u), y);
+                      const uint32_t sh = cvt_e4m3x2(sb[c][r][w / 2] & ((ta + 8 * r < see ? 0xffu : 0u) | (tb + 8 * r < see ? 0xff00u : 0u)));
+                      f[2 * r] = hmul2(x[j], sh);
+                      f[2 * r + 1] = hmul2(y[j], sh);
+                    }
+                    float* acc = o[n][4 * w + j];
+                    float t[4] = {acc[0], acc[1], acc[2], acc[3]};
+                    mma_f16(t, f[0], f[1], f[2], f[3], pb[c][n][0], pb[c][n][1]);
+                    if (col == 2 * qd) { acc[0] = t[0]; acc[2] = t[2]; }
+                    if (col == 2 * qd + 1) { acc[1] = t[1]; acc[3] = t[3]; }
+                  }
+                }
               }
             }
           }
         }
       }
-      if (here) phase ^= 1u << slot;
+      if (here != 0) phase ^= 1u << slot;
       __syncwarp();                                 // the slot has been read by every lane
       produce();
       slot = slot + 1 == ST ? 0 : slot + 1;
@@ -563,8 +619,9 @@ kv_attention_kernel(const AttnArgs a) {
         if (f != 0.f) { acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f; }
       }
       if (whole) {
-        const int r = row0 + row, tok = r / a.group;
-        const int64_t at = static_cast<int64_t>(cc.r.q0 + tok) * (a.heads * a.group) + cc.h * a.group + r % a.group;
+        uint32_t tok, hd;
+        a.group_div.divmod(row0 + row, tok, hd);
+        const int64_t at = static_cast<int64_t>(cc.r.q0 + tok) * (a.heads * a.group) + cc.h * a.group + hd;
         const float f = ll == 0.f ? 0.f : __fdividef(v2, ll);
         uint2 packed;
         packed.x = Elem<T>::pack2(acc[0] * f, acc[1] * f);
@@ -582,10 +639,12 @@ kv_attention_kernel(const AttnArgs a) {
       const int64_t owner = ((seg_last + 1) * ctas - 1) / total;
       my_desc = make_int4(cc.b, cc.h, cc.rt, static_cast<int>(owner - cta + 1));
     }
-    __syncthreads();
     left -= kt_end - cc.kt;
-    cc.kt = kt_end;
-    if (left > 0) next_segment<RT>(a, cc);
+    __syncthreads();
+    if (left > 0) {
+      if (threadIdx.x == 0) next_segment<RT>(a, cc);
+      __syncthreads();
+    }
   }
   if (threadIdx.x == 0) a.desc[cta] = my_desc;
   grace_after_abort(&abort_flag);
@@ -716,6 +775,8 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
   a.width = width; a.requests = requests; a.tokens = tokens; a.heads = heads; a.group = group;
   a.page = page; a.pages = pages; a.zero_tail = cu_q ? zero_tail : 0;
   a.scale = scale;
+  a.chunks_per_page = FastDiv(page / kChunk);
+  a.group_div = FastDiv(group);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto go = [&](auto t) {
     using T = decltype(t);
