@@ -4,9 +4,9 @@
 // over the tokens j that query t of its request sees (its own position and everything before it).
 //
 // Work.  A segment is one kv head of one request and one tile of 8 NT query rows (query tokens x the heads
-// that share the kv head); its cache tokens are cut into tiles of 128.  All tiles of all segments form one line
-// that is dealt out to the CTAs in equal contiguous shares, so ragged lengths balance without the host knowing
-// a length.  A segment that lies inside one share is finished there; pieces of the others go to a workspace as
+// that share the kv head); its cache tokens are cut into tiles of 128.  All tiles of all segments, each segment
+// preceded by kSegCost units for beginning and ending it, form one line that is dealt out to the CTAs in equal
+// contiguous shares, so ragged lengths balance without the host knowing a length.  A segment that lies inside one share is finished there; pieces of the others go to a workspace as
 // (max, sum, unnormalised output) and kv_merge_kernel joins them in a fixed order.
 //
 // Inside a CTA the four warps take 32 tokens of each tile.  A warp's codes and scales come by four bulk copies
@@ -32,6 +32,7 @@ constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kChunk = 16;                          // tokens of a matrix product
 constexpr int kStep = 2 * kChunk;                   // tokens a warp handles at a time
 constexpr int kTile = kStep * kAttnWarps;           // tokens of a tile
+constexpr int kSegCost = 2;                         // what beginning and ending a segment costs, in tiles
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kAttnWaitCode = 1u << 20;
 
@@ -77,7 +78,7 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int b) {
   return r;
 }
 __device__ __forceinline__ int64_t request_work(const AttnArgs& a, const Request& r) {
-  return static_cast<int64_t>(a.heads) * r.nrt * r.nkt;
+  return static_cast<int64_t>(a.heads) * r.nrt * (r.nkt + kSegCost);
 }
 
 // a place on the line of tiles
@@ -173,7 +174,8 @@ struct AttnShape {
   static constexpr int kCtas = D * NT >= 256 ? 2 : 4;                  // per SM
 };
 
-template <typename T, int D, int NT>
+// kRagged: requests may have several queries (cu_q), so that rows of a tile may see different tokens.
+template <typename T, int D, int NT, bool kRagged>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas)
 kv_attention_kernel(const AttnArgs a) {
   using S = AttnShape<D, NT>;
@@ -186,6 +188,7 @@ kv_attention_kernel(const AttnArgs a) {
   __shared__ __align__(8) uint64_t bars[kAttnWarps * ST];
   __shared__ int64_t scan_sums[kAttnWarps];
   __shared__ Cursor cc, pcs[kAttnWarps];            // where the CTA's products and each warp's copies are: read between segments only
+  __shared__ int start_unit;                        // of the first segment
   __shared__ uint32_t abort_flag;
   __shared__ float2 merge_ml[kAttnWarps][RT];
 
@@ -216,7 +219,7 @@ kv_attention_kernel(const AttnArgs a) {
     if (w < warp) before += scan_sums[w];
     total += scan_sums[w];
   }
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total), cta = blockIdx.x;
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total / (kSegCost + 1)), cta = blockIdx.x;
   if (cta >= ctas) {
     if (threadIdx.x == 0) a.desc[cta] = make_int4(0, 0, 0, 0);
     return;
@@ -232,8 +235,10 @@ kv_attention_kernel(const AttnArgs a) {
       at += w;
     }
     const int64_t in = t0 - at;
-    c.kt = static_cast<int>(in % c.r.nkt);
-    const int64_t seg = in / c.r.nkt;
+    const int units = c.r.nkt + kSegCost;           // the first kSegCost units of a segment hold no tile
+    const int64_t seg = in / units;
+    start_unit = static_cast<int>(in % units);
+    c.kt = max(start_unit - kSegCost, 0);
     c.rt = static_cast<int>(seg % c.r.nrt);
     c.h = static_cast<int>(seg / c.r.nrt);
     cc = c;
@@ -243,69 +248,62 @@ kv_attention_kernel(const AttnArgs a) {
   __syncthreads();
 
   // ---- the warp's producer: bulk copies of 32 tokens into a ring of its own ----
+  // Lanes 0 to 3 fetch the codes of K and V and the scales of K and V, each from a base pointer of its own.
   uint8_t* ring = smem + warp * ST * S::kSlot;
   uint64_t* bar = bars + warp * ST;
   const bool wide = a.page % kStep == 0;            // the 32 tokens of a step lie in one page
+  const uint8_t* my_src = lane == 0 ? a.k_codes : lane == 1 ? a.v_codes : lane == 2 ? a.k_scales : a.v_scales;
+  const int my_unit = lane < 2 ? D / 2 : D / 16;    // bytes of a token
+  uint8_t* my_dst = ring + (lane < 2 ? lane * S::kCodeBytes : 2 * S::kCodeBytes + (lane - 2) * S::kScaleBytes);
   Cursor& pc = pcs[warp];
-  int p_kt = pc.kt, p_nkt = pc.r.nkt, p_head = pc.h;
+  int p_tok = pc.kt * kTile + warp * kStep, p_end = pc.r.nkt * kTile, p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
+  int p_left = static_cast<int>(t1 - t0) - max(kSegCost - start_unit, 0);
   const int* p_row = a.table + pc.b * a.table_stride;
-  int64_t p_left = t1 - t0;
+  const uint8_t* p_src = my_src + static_cast<int64_t>(pc.h) * a.page * my_unit;
+  const int64_t page_bytes = static_cast<int64_t>(a.heads) * a.page * my_unit;
+  const int p_left0 = p_left;                       // tiles and segment costs of the share
   uint32_t live = 0, phase = 0;                     // bits 2s, 2s + 1: the halves of slot s that hold (or await) tokens; parities
-  int p_slot = 0, p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
-  int p_id[2], p_in[2];                             // page ids of the step's halves (-1: nothing to read), tokens into the page
-  auto look_up = [&]() {
+  int p_slot = 0;
+  int p_id[2], p_in[2];                             // page ids of the step's halves (negative: nothing to read), tokens into the page
+  auto look_up = [&]() {                            // the ids are not looked at before the next step: their latency is hidden
     p_id[0] = p_id[1] = -1;
-    const int tok = p_kt * kTile + warp * kStep;
-    if (p_left <= 0 || tok >= p_limit) return;
+    if (p_left <= 0 || p_tok >= p_limit) return;
     uint32_t col, in;
-    a.chunks_per_page.divmod(tok / kChunk, col, in);
-    int id = __ldg(p_row + col);
-    p_id[0] = id < a.pages ? id : -1;
+    a.chunks_per_page.divmod(p_tok / kChunk, col, in);
     p_in[0] = in * kChunk;
-    if (tok + kChunk < p_limit) {
-      p_in[1] = p_in[0] + kChunk;
-      if (!wide && ++in == a.chunks_per_page.d) {   // the second half begins the next page
-        id = __ldg(p_row + col + 1);
-        p_in[1] = 0;
-      }
-      p_id[1] = id < a.pages ? id : -1;
+    p_id[0] = __ldg(p_row + col);
+    if (p_tok + kChunk < p_limit) {
+      const bool next = !wide && in + 1 == a.chunks_per_page.d;                    // the second half begins the next page
+      p_in[1] = next ? 0 : p_in[0] + kChunk;
+      p_id[1] = __ldg(p_row + col + next);
     }
   };
   look_up();
   auto produce = [&]() {
-    const bool ok0 = p_id[0] >= 0, ok1 = p_id[1] >= 0;
-    if (lane == 0 && (ok0 || ok1)) {
-      uint8_t* dst = ring + p_slot * S::kSlot;
+    const bool ok0 = static_cast<uint32_t>(p_id[0]) < static_cast<uint32_t>(a.pages);
+    const bool ok1 = static_cast<uint32_t>(p_id[1]) < static_cast<uint32_t>(a.pages);
+    if (lane < 4 && (ok0 || ok1)) {
       uint64_t* b = bar + p_slot;
-      mbar_expect_tx(b, ok0 && ok1 ? S::kSlot : S::kSlot / 2);
-      auto copy = [&](int half, int id, int in, int share) {                       // 1 / share of a slot
-        const int64_t row = (static_cast<int64_t>(id) * a.heads + p_head) * a.page + in;
-        uint8_t* c = dst + half * (S::kCodeBytes / 2);
-        uint8_t* s = dst + 2 * S::kCodeBytes + half * (S::kScaleBytes / 2);
-        bulk_load(c, a.k_codes + row * (D / 2), S::kCodeBytes / share, b);
-        bulk_load(c + S::kCodeBytes, a.v_codes + row * (D / 2), S::kCodeBytes / share, b);
-        bulk_load(s, a.k_scales + row * (D / 16), S::kScaleBytes / share, b);
-        bulk_load(s + S::kScaleBytes, a.v_scales + row * (D / 16), S::kScaleBytes / share, b);
-      };
-      if (wide && ok1) {
-        copy(0, p_id[0], p_in[0], 1);
+      uint8_t* dst = my_dst + p_slot * S::kSlot;
+      if (lane == 0) mbar_expect_tx(b, ok0 && ok1 ? S::kSlot : S::kSlot / 2);
+      if (wide) {
+        bulk_load(dst, p_src + p_id[0] * page_bytes + p_in[0] * my_unit, (ok1 ? kStep : kChunk) * my_unit, b);
       } else {
-        if (ok0) copy(0, p_id[0], p_in[0], 2);
-        if (ok1) copy(1, p_id[1], p_in[1], 2);
+        if (ok0) bulk_load(dst, p_src + p_id[0] * page_bytes + p_in[0] * my_unit, kChunk * my_unit, b);
+        if (ok1) bulk_load(dst + kChunk * my_unit, p_src + p_id[1] * page_bytes + p_in[1] * my_unit, kChunk * my_unit, b);
       }
     }
     live = (live & ~(3u << (2 * p_slot))) | ((ok0 ? 1u : 0u) | (ok1 ? 2u : 0u)) << (2 * p_slot);
     p_slot = p_slot + 1 == ST ? 0 : p_slot + 1;
-    if (--p_left > 0) {
-      if (++p_kt == p_nkt) {
-        if (lane == 0) next_segment<RT>(a, pc);
-        __syncwarp();
-        p_kt = 0;
-        p_nkt = pc.r.nkt;
-        p_head = pc.h;
-        p_row = a.table + pc.b * a.table_stride;
-        p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
-      }
+    p_tok += kTile;
+    if (--p_left > 0 && p_tok >= p_end && (p_left -= kSegCost) > 0) {
+      if (lane == 0) next_segment<RT>(a, pc);
+      __syncwarp();
+      p_tok = warp * kStep;
+      p_end = pc.r.nkt * kTile;
+      p_row = a.table + pc.b * a.table_stride;
+      p_src = my_src + static_cast<int64_t>(pc.h) * a.page * my_unit;
+      p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
     }
     look_up();
   };
@@ -313,19 +311,18 @@ kv_attention_kernel(const AttnArgs a) {
   for (int s = 0; s < ST; ++s) produce();
 
   const float qk = a.scale * kLog2e * __ldg(a.k_scale2), v2 = __ldg(a.v_scale2);
-  int64_t left = t1 - t0;
+  int left = p_left0;
   int slot = 0;
   int4 my_desc = make_int4(0, 0, 0, 0);
 
   while (left > 0) {
     // ---- one segment, or this CTA's part of it ----
-    const int kt_end = static_cast<int>(min(static_cast<int64_t>(cc.r.nkt), cc.kt + left));
+    const int kt_end = min(cc.r.nkt, cc.kt + left);
     const int row0 = cc.rt * RT, rows = min(cc.r.nq * a.group - row0, RT);
     const int lim_lo = row_limit(a, cc.r, row0), lim_hi = row_limit(a, cc.r, row0 + rows - 1);
     // queries: thread (gr, qd) holds dimensions qd * D/4 ... of row gr of each 8-row tile, as fp16 times 2^k
     uint32_t qf[NT][D / 8];
     float qs[NT][2];
-    int lim[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 8 * n + gr;
@@ -362,7 +359,6 @@ kv_attention_kernel(const AttnArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {                 // of the rows this thread's accumulators belong to
         qs[n][j] = qk * __shfl_sync(0xffffffffu, back, 4 * (2 * qd + j));
-        lim[n][j] = row_limit(a, cc.r, row0 + 8 * n + 2 * qd + j);
       }
     }
     float o[NT][D / 16][4];
@@ -430,6 +426,20 @@ kv_attention_kernel(const AttnArgs a) {
         }
         // ---- softmax, base 2 ----
         const bool masked = tok0 + kStep > lim_lo || here != 3u;
+        uint32_t hidden = 0;                        // bit 8 n + 4 c + j: that score is masked
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int see = row_limit(a, cc.r, row0 + 8 * n + 2 * qd + j) - tok0 - tg;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (c * kChunk >= see || !(here >> c & 1u)) hidden |= 1u << (8 * n + 4 * c + j);
+                if (c * kChunk + 8 >= see || !(here >> c & 1u)) hidden |= 1u << (8 * n + 4 * c + j + 2);
+              }
+            }
+        }
         bool grow = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -437,10 +447,10 @@ kv_attention_kernel(const AttnArgs a) {
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[c][n][j] *= qs[n][j & 1];
-            if (masked) {
+            if (hidden) {
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                if (tok0 + c * kChunk + tg + 8 * (j >> 1) >= lim[n][j & 1] || !(here >> c & 1u)) s[c][n][j] = -INFINITY;
+                if (hidden >> (8 * n + 4 * c + j) & 1u) s[c][n][j] = -INFINITY;
             }
           }
 #pragma unroll
@@ -502,10 +512,11 @@ kv_attention_kernel(const AttnArgs a) {
                 const bool on = here >> c & 1u;
                 sb[c][r][i] &= (on && t + ta < lim_hi ? 0xffu : 0u) | (on && t + tb < lim_hi ? 0xff00u : 0u);
                 // some rows see tokens that others do not
-                nan_v |= lim_lo < lim_hi && ((sb[c][r][i] & 0x7fu) == 0x7fu || (sb[c][r][i] & 0x7f00u) == 0x7f00u);
+                if constexpr (kRagged)
+                  nan_v |= lim_lo < lim_hi && ((sb[c][r][i] & 0x7fu) == 0x7fu || (sb[c][r][i] & 0x7f00u) == 0x7f00u);
               }
         }
-        if (!masked || !__any_sync(0xffffffffu, nan_v)) {
+        if (!kRagged || !masked || !__any_sync(0xffffffffu, nan_v)) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t wa[2][VW], wb[2][VW], sh[2][VB];
@@ -533,7 +544,7 @@ kv_attention_kernel(const AttnArgs a) {
                   mma_f16(o[n][4 * w + j], x[0][j], y[0][j], x[1][j], y[1][j], pb[c][n][0], pb[c][n][1]);
             }
           }
-        } else {
+        } else if constexpr (kRagged) {
           // A NaN value that only some rows may see: each row's product on its own, with what it does not see
           // zeroed, and only that row's column kept.
 #pragma unroll
@@ -639,7 +650,7 @@ kv_attention_kernel(const AttnArgs a) {
       const int64_t owner = ((seg_last + 1) * ctas - 1) / total;
       my_desc = make_int4(cc.b, cc.h, cc.rt, static_cast<int>(owner - cta + 1));
     }
-    left -= kt_end - cc.kt;
+    left -= kt_end - cc.kt + kSegCost;
     __syncthreads();
     if (left > 0) {
       if (threadIdx.x == 0) next_segment<RT>(a, cc);
@@ -709,7 +720,7 @@ kv_merge_kernel(const AttnArgs a) {
 template <typename T, int D, int NT>
 int launch_attention(const AttnArgs& a, int ctas, cudaStream_t s) {
   using S = AttnShape<D, NT>;
-  auto kern = kv_attention_kernel<T, D, NT>;
+  auto kern = a.cu_q ? kv_attention_kernel<T, D, NT, true> : kv_attention_kernel<T, D, NT, false>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
   launch_pdl(kern, ctas, kAttnThreads, S::kSmem, s, a);
   launch_pdl(kv_merge_kernel<T, D, S::kRT>, dim3(ctas, S::kRT), 128, 0, s, a);
@@ -751,7 +762,7 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
   if (!cu_q && tokens != requests) return B200Q_ERR_SHAPE;
   if (dim != 64 && dim != 128 && dim != 256) return B200Q_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(tokens) * group > kFastDivLimit / 2 || static_cast<int64_t>(heads) * group > kFastDivLimit ||
-      static_cast<int64_t>(width) * page > (1ll << 40))
+      static_cast<int64_t>(width) * page > (1 << 30))
     return B200Q_ERR_UNSUPPORTED;
   const uintptr_t align = reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(2 * q_token_stride) |
                           static_cast<uintptr_t>(2 * q_head_stride) | reinterpret_cast<uintptr_t>(k_codes) |
