@@ -522,14 +522,14 @@ int b200q_nvfp4_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_
  * logarithm) or NULL.  dim 64, 128 or 256; page a multiple of 16; table rows as in b200q_kv_step (an id outside
  * [0, pages) hides its tokens; lens beyond width * page are cut).  Rows of q at and behind cu_q[requests] are not
  * computed: their output is left as it is, or zeroed (lse -inf) where zero_tail != 0.
- * workspace: b200q_nvfp4_kv_attention_workspace(...) bytes, this call's alone until it has run; *status_io as in
- * b200q_fp8_gemm.  Lengths are read on the device only: the call can be captured and replayed with others. */
+ * workspace: b200q_nvfp4_kv_attention_workspace(...) bytes, this call's alone until it has run.  Lengths are read on the
+ * device only: the call can be captured and replayed with others.  width * page at most 2^30. */
 int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
                              const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
                              const uint8_t* v_scales, const float* k_scale2, const float* v_scale2, const int* table,
                              int64_t table_stride, int width, const int* lens, const int* cu_q, int requests, int tokens,
                              int heads, int group, int dim, int pages, int page, float scale, void* out, float* lse,
-                             int zero_tail, void* workspace, int64_t workspace_bytes, uint32_t* status_io, void* stream);
+                             int zero_tail, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t b200q_nvfp4_kv_attention_workspace(int tokens, int requests, int heads, int group, int dim);
 
 /* ---------------------------------------------------------------- export packers ------------ */

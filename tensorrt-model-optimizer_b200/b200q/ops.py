@@ -1088,7 +1088,7 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
              block_table.stride(0) if b > 1 else block_table.shape[1], block_table.shape[1], lens.data_ptr(),
              cu_q.data_ptr() if cu_q is not None else None, b, tokens, heads, group, dim, pages, page,
              dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr() if return_lse else None,
-             int(zero_tail), ws.data_ptr(), need, qgemm_status(dev).data_ptr(), _stream(q))
+             int(zero_tail), ws.data_ptr(), need, _stream(q))
     return (out, lse) if return_lse else out
 
 

@@ -9,10 +9,9 @@
 // contiguous shares, so ragged lengths balance without the host knowing a length.  A segment that lies inside one share is finished there; pieces of the others go to a workspace as
 // (max, sum, unnormalised output) and kv_merge_kernel joins them in a fixed order.
 //
-// Inside a CTA the four warps take 32 tokens of each tile.  A warp's codes and scales come by four bulk copies
-// per 32 tokens (2 KB + 256 B each for K and V at D = 128; per 16 tokens where pages are not multiples of 32) into a
-// ring of its own, two steps deep, with the page ids read ahead; there is no block-wide barrier before the end of a
-// segment.
+// Inside a CTA the four warps take 32 tokens of each tile.  A warp fetches its codes and scales (2 KB + 256 B each for
+// K and V at D = 128) with cp.async into a ring of its own, two steps deep, with the page ids read ahead; there is no
+// block-wide barrier before the end of a segment.
 //
 // Mathematics.  S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: cache tokens (or head dimensions) fill the 16
 // rows, the query rows the 8 columns, so a group of up to eight heads wastes nothing.  E2M1 times E4M3 has at
@@ -34,7 +33,6 @@ constexpr int kStep = 2 * kChunk;                   // tokens a warp handles at 
 constexpr int kTile = kStep * kAttnWarps;           // tokens of a tile
 constexpr int kSegCost = 2;                         // what beginning and ending a segment costs, in tiles
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr uint32_t kAttnWaitCode = 1u << 20;
 
 struct AttnArgs {
   const void* q;
@@ -50,7 +48,6 @@ struct AttnArgs {
   float* part;                                      // [ctas, 2, rows, D]
   float2* part_ml;                                  // [ctas, 2, rows]
   int4* desc;                                       // [ctas]: request, head, row tile, pieces
-  uint32_t* status;
   FastDiv chunks_per_page, group_div;
   int width, requests, tokens, heads, group, page, pages, zero_tail;
   float scale;
@@ -139,6 +136,9 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -185,19 +185,12 @@ kv_attention_kernel(const AttnArgs a) {
   constexpr int VW = D / 64;                        // words of codes a thread reads of one V token
   constexpr int VB = D >= 128 ? D / 128 : 1;        // block scales of them
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kAttnWarps * ST];
   __shared__ int64_t scan_sums[kAttnWarps];
   __shared__ Cursor cc, pcs[kAttnWarps];            // where the CTA's products and each warp's copies are: read between segments only
   __shared__ int start_unit;                        // of the first segment
-  __shared__ uint32_t abort_flag;
   __shared__ float2 merge_ml[kAttnWarps][RT];
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
-  if (threadIdx.x < kAttnWarps * ST) mbar_init(&bars[threadIdx.x], 1);
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   pdl_prologue();
 
   // ---- this CTA's share of the line of tiles ----
@@ -247,22 +240,20 @@ kv_attention_kernel(const AttnArgs a) {
   }
   __syncthreads();
 
-  // ---- the warp's producer: bulk copies of 32 tokens into a ring of its own ----
-  // Lanes 0 to 3 fetch the codes of K and V and the scales of K and V, each from a base pointer of its own.
+  // ---- the warp's producer: cp.async of 32 tokens into a ring of its own ----
+  constexpr int kSide = D / 16;                     // lanes that fetch a chunk's scales of one side, 16 bytes each
   uint8_t* ring = smem + warp * ST * S::kSlot;
-  uint64_t* bar = bars + warp * ST;
-  const bool wide = a.page % kStep == 0;            // the 32 tokens of a step lie in one page
-  const uint8_t* my_src = lane == 0 ? a.k_codes : lane == 1 ? a.v_codes : lane == 2 ? a.k_scales : a.v_scales;
-  const int my_unit = lane < 2 ? D / 2 : D / 16;    // bytes of a token
-  uint8_t* my_dst = ring + (lane < 2 ? lane * S::kCodeBytes : 2 * S::kCodeBytes + (lane - 2) * S::kScaleBytes);
+  const uint32_t ring_addr = smem_u32(ring) + lane * 16;
+  const uint32_t scale_addr = smem_u32(ring) + 2 * S::kCodeBytes + (lane < kSide ? lane * 16 : S::kScaleBytes + (lane - kSide) * 16);
+  const uint8_t* scale_src = lane < kSide ? a.k_scales + lane * 16 : a.v_scales + (lane - kSide) * 16;
   Cursor& pc = pcs[warp];
   int p_tok = pc.kt * kTile + warp * kStep, p_end = pc.r.nkt * kTile, p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
   int p_left = static_cast<int>(t1 - t0) - max(kSegCost - start_unit, 0);
-  const int* p_row = a.table + pc.b * a.table_stride;
-  const uint8_t* p_src = my_src + static_cast<int64_t>(pc.h) * a.page * my_unit;
-  const int64_t page_bytes = static_cast<int64_t>(a.heads) * a.page * my_unit;
   const int p_left0 = p_left;                       // tiles and segment costs of the share
-  uint32_t live = 0, phase = 0;                     // bits 2s, 2s + 1: the halves of slot s that hold (or await) tokens; parities
+  const int* p_row = a.table + pc.b * a.table_stride;
+  int p_head = pc.h * a.page;
+  const int page_tokens = a.heads * a.page;
+  uint32_t live = 0;                                // bits 2s, 2s + 1: the halves of slot s that hold (or await) tokens
   int p_slot = 0;
   int p_id[2], p_in[2];                             // page ids of the step's halves (negative: nothing to read), tokens into the page
   auto look_up = [&]() {                            // the ids are not looked at before the next step: their latency is hidden
@@ -273,27 +264,32 @@ kv_attention_kernel(const AttnArgs a) {
     p_in[0] = in * kChunk;
     p_id[0] = __ldg(p_row + col);
     if (p_tok + kChunk < p_limit) {
-      const bool next = !wide && in + 1 == a.chunks_per_page.d;                    // the second half begins the next page
+      const bool next = in + 1 == a.chunks_per_page.d;                             // the second half begins the next page
       p_in[1] = next ? 0 : p_in[0] + kChunk;
       p_id[1] = __ldg(p_row + col + next);
     }
   };
   look_up();
   auto produce = [&]() {
-    const bool ok0 = static_cast<uint32_t>(p_id[0]) < static_cast<uint32_t>(a.pages);
-    const bool ok1 = static_cast<uint32_t>(p_id[1]) < static_cast<uint32_t>(a.pages);
-    if (lane < 4 && (ok0 || ok1)) {
-      uint64_t* b = bar + p_slot;
-      uint8_t* dst = my_dst + p_slot * S::kSlot;
-      if (lane == 0) mbar_expect_tx(b, ok0 && ok1 ? S::kSlot : S::kSlot / 2);
-      if (wide) {
-        bulk_load(dst, p_src + p_id[0] * page_bytes + p_in[0] * my_unit, (ok1 ? kStep : kChunk) * my_unit, b);
-      } else {
-        if (ok0) bulk_load(dst, p_src + p_id[0] * page_bytes + p_in[0] * my_unit, kChunk * my_unit, b);
-        if (ok1) bulk_load(dst + kChunk * my_unit, p_src + p_id[1] * page_bytes + p_in[1] * my_unit, kChunk * my_unit, b);
+    uint32_t ok = 0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (static_cast<uint32_t>(p_id[c]) < static_cast<uint32_t>(a.pages)) {
+        ok |= 1u << c;
+        const int64_t row = static_cast<int64_t>(p_id[c]) * page_tokens + (p_head + p_in[c]);
+        const uint8_t* ksrc = a.k_codes + row * (D / 2) + lane * 16;
+        const uint8_t* vsrc = a.v_codes + row * (D / 2) + lane * 16;
+        const uint32_t dst = ring_addr + p_slot * S::kSlot + c * (S::kCodeBytes / 2);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          copy_async16(dst + i * 512, ksrc + i * 512);
+          copy_async16(dst + S::kCodeBytes + i * 512, vsrc + i * 512);
+        }
+        if (lane < 2 * kSide) copy_async16(scale_addr + p_slot * S::kSlot + c * (S::kScaleBytes / 2), scale_src + row * (D / 16));
       }
     }
-    live = (live & ~(3u << (2 * p_slot))) | ((ok0 ? 1u : 0u) | (ok1 ? 2u : 0u)) << (2 * p_slot);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    live = (live & ~(3u << (2 * p_slot))) | ok << (2 * p_slot);
     p_slot = p_slot + 1 == ST ? 0 : p_slot + 1;
     p_tok += kTile;
     if (--p_left > 0 && p_tok >= p_end && (p_left -= kSegCost) > 0) {
@@ -302,7 +298,7 @@ kv_attention_kernel(const AttnArgs a) {
       p_tok = warp * kStep;
       p_end = pc.r.nkt * kTile;
       p_row = a.table + pc.b * a.table_stride;
-      p_src = my_src + static_cast<int64_t>(pc.h) * a.page * my_unit;
+      p_head = pc.h * a.page;
       p_limit = row_limit(a, pc.r, pc.rt * RT + RT - 1);
     }
     look_up();
@@ -380,10 +376,9 @@ kv_attention_kernel(const AttnArgs a) {
 #pragma unroll 1
     for (int kt = cc.kt; kt < kt_end; ++kt) {
       const uint32_t here = (live >> (2 * slot)) & 3u;
-      const bool landed = here != 0 && __all_sync(0xffffffffu, mbar_wait_bounded(bar + slot, (phase >> slot) & 1u, &abort_flag,
-                                                                                 a.status, kAttnWaitCode));
-      if (here != 0 && !landed) p_left = 0;         // gave up: nothing more is asked for
-      if (landed) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+      __syncwarp();                                 // every lane's part of the slot has landed
+      if (here != 0) {
         const uint8_t* kc = ring + slot * S::kSlot;
         const uint8_t* vc = kc + S::kCodeBytes;
         const uint8_t* ks = kc + 2 * S::kCodeBytes;
@@ -586,7 +581,6 @@ kv_attention_kernel(const AttnArgs a) {
           }
         }
       }
-      if (here != 0) phase ^= 1u << slot;
       __syncwarp();                                 // the slot has been read by every lane
       produce();
       slot = slot + 1 == ST ? 0 : slot + 1;
@@ -658,7 +652,7 @@ kv_attention_kernel(const AttnArgs a) {
     }
   }
   if (threadIdx.x == 0) a.desc[cta] = my_desc;
-  grace_after_abort(&abort_flag);
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Pieces of the segments that span several CTAs, joined in the order of the CTAs.  Block (c, row): the segment
@@ -751,10 +745,10 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
                                         const int* table, int64_t table_stride, int width, const int* lens, const int* cu_q,
                                         int requests, int tokens, int heads, int group, int dim, int pages, int page,
                                         float scale, void* out, float* lse, int zero_tail, void* workspace,
-                                        int64_t workspace_bytes, uint32_t* status_io, void* stream) {
+                                        int64_t workspace_bytes, void* stream) {
   B200Q_REQUIRE_PTR(q); B200Q_REQUIRE_PTR(k_codes); B200Q_REQUIRE_PTR(k_scales); B200Q_REQUIRE_PTR(v_codes);
   B200Q_REQUIRE_PTR(v_scales); B200Q_REQUIRE_PTR(k_scale2); B200Q_REQUIRE_PTR(v_scale2); B200Q_REQUIRE_PTR(lens);
-  B200Q_REQUIRE_PTR(out); B200Q_REQUIRE_PTR(workspace); B200Q_REQUIRE_PTR(status_io);
+  B200Q_REQUIRE_PTR(out); B200Q_REQUIRE_PTR(workspace);
   if (width > 0) B200Q_REQUIRE_PTR(table);
   if (dtype != B200Q_F16 && dtype != B200Q_BF16) return B200Q_ERR_DTYPE;
   if (requests <= 0 || tokens <= 0 || heads <= 0 || group <= 0 || pages <= 0 || width < 0 || table_stride < 0) return B200Q_ERR_SHAPE;
@@ -782,7 +776,6 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
   a.desc = static_cast<int4*>(workspace);
   a.part = reinterpret_cast<float*>(a.desc + ctas);
   a.part_ml = reinterpret_cast<float2*>(a.part + static_cast<int64_t>(ctas) * 2 * 8 * nt * dim);
-  a.status = status_io;
   a.width = width; a.requests = requests; a.tokens = tokens; a.heads = heads; a.group = group;
   a.page = page; a.pages = pages; a.zero_tail = cu_q ? zero_tail : 0;
   a.scale = scale;

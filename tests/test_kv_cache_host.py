@@ -59,11 +59,11 @@ def test_status_codes():
     def attention(**kw):
         a = dict(q=p, qs=64, qh=64, dtype=2, kc=p, ks=p, vc=p, vs=p, k2=p, v2=p, table=p, stride=1, width=1, lens=p, cu=None,
                  requests=1, tokens=1, heads=1, group=1, dim=64, pages=1, page=16, scale=1.0, out=p, lse=None, tail=1, ws=p,
-                 ws_bytes=1 << 40, status=p)
+                 ws_bytes=1 << 40)
         a.update(kw)
         return lib.b200q_nvfp4_kv_attention(*a.values(), None)
 
-    for name in ("q", "kc", "ks", "vc", "vs", "k2", "v2", "table", "lens", "out", "ws", "status"):
+    for name in ("q", "kc", "ks", "vc", "vs", "k2", "v2", "table", "lens", "out", "ws"):
         assert attention(**{name: None}) == NULL, name
     assert attention(dtype=0) == DTYPE
     for kw in (dict(requests=0), dict(tokens=2), dict(heads=0), dict(group=0), dict(pages=0), dict(page=24), dict(stride=-1), dict(width=-1)):
