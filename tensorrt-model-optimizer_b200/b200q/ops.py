@@ -54,7 +54,8 @@ def _on(device):
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """Handle of torch's current stream on t's device (without building the ``Stream`` object, which costs 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _amax_f32(amax: torch.Tensor, device) -> torch.Tensor:
@@ -940,7 +941,7 @@ def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor
         raise ValueError("b200q: the rows of block_table overlap")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
     ints = torch.empty(2 * b + 3 + tokens, dtype=torch.int32, device=dev)
-    cu, lens_out, taken_out, status, positions = ints.split((b + 1, b, 1, 1, tokens))
+    cu, lens_out, taken_out, status, positions = ints.split_with_sizes((b + 1, b, 1, 1, tokens))
     at = ints.data_ptr()
     with _on(dev):
         call("b200q_kv_step", lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(),
@@ -954,7 +955,7 @@ def _kv_pages(cache, what: str, device=None):
     """(codes, scales) of one side of a cache, checked -> (codes, scales, pages, heads, page size, dim)."""
     codes, scales = cache
     _cuda(codes, what), _cuda(scales, what)
-    if codes.dim() != 4 or scales.dim() != 4 or codes.dtype != torch.uint8 or scales.element_size() != 1:
+    if codes.dim() != 4 or codes.dtype != torch.uint8 or scales.element_size() != 1:
         raise ValueError(f"b200q: {what} must be (codes uint8 [pages, heads, page, dim/2], scales float8_e4m3fn "
                          "[pages, heads, page, dim/16])")
     pages, heads, page, half = codes.shape
@@ -1025,6 +1026,11 @@ def nvfp4_kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cac
 _KV_DIMS = (64, 128, 256)
 
 
+@functools.lru_cache(maxsize=4096)
+def _kv_attention_workspace(device: int, *sizes: int) -> int:
+    return call("b200q_nvfp4_kv_attention_workspace", *sizes)
+
+
 def nvfp4_kv_attention_supported(q: torch.Tensor, heads: int, page: int) -> bool:
     """Whether ``nvfp4_kv_attention`` covers q [tokens, query heads, dim] over a cache of ``heads`` kv heads."""
     return (q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and q.shape[2] in _KV_DIMS
@@ -1081,7 +1087,7 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
     k2, v2 = _kv_scale2(k_scale2, dev), _kv_scale2(v_scale2, dev)
     group = qheads // heads
     with _on(dev):
-        need = call("b200q_nvfp4_kv_attention_workspace", tokens, b, heads, group, dim)
+        need = _kv_attention_workspace(dev.index, tokens, b, heads, group, dim)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)   # this call's own: the allocator orders its reuse
         call("b200q_nvfp4_kv_attention", q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q), kc.data_ptr(), ks.data_ptr(),
              vc.data_ptr(), vs.data_ptr(), k2.data_ptr(), v2.data_ptr(), block_table.data_ptr(),

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/b200q.h"
@@ -61,6 +62,18 @@ __device__ __forceinline__ void pdl_prologue() {
 #endif
 
 int sm_count_cached();
+
+// Raises a kernel's dynamic shared memory limit once per device; `done` is a static of the caller's, one per kernel.
+// (The runtime call costs as much host time as a small launch.)
+inline bool allow_smem(const void* kern, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) return false;
+  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return true;
+}
 
 // Dispatch a generic lambda on the element type.
 #define B200Q_DISPATCH(dtype, ...)                         \

@@ -715,7 +715,8 @@ template <typename T, int D, int NT>
 int launch_attention(const AttnArgs& a, int ctas, cudaStream_t s) {
   using S = AttnShape<D, NT>;
   auto kern = a.cu_q ? kv_attention_kernel<T, D, NT, true> : kv_attention_kernel<T, D, NT, false>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
+  static std::atomic<uint64_t> done[2];
+  if (!allow_smem(reinterpret_cast<const void*>(kern), S::kSmem, done[a.cu_q ? 1 : 0])) return B200Q_ERR_CUDA;
   launch_pdl(kern, ctas, kAttnThreads, S::kSmem, s, a);
   launch_pdl(kv_merge_kernel<T, D, S::kRT>, dim3(ctas, S::kRT), 128, 0, s, a);
   return launch_status();

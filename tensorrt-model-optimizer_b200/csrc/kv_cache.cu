@@ -209,8 +209,8 @@ extern "C" int b200q_kv_step(const int* lens, const int* new_lens, const int* fr
   if (requests <= 0 || page <= 0 || tokens < 0 || nfree < 0 || width < 0 || table_stride < width) return B200Q_ERR_SHAPE;
   if (requests > kStepMaxRequests || tokens > (1 << 30)) return B200Q_ERR_UNSUPPORTED;
   const size_t smem = sizeof(int) * (3 * static_cast<size_t>(requests) + 2);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kv_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+  static std::atomic<uint64_t> done;
+  if (smem > 48 * 1024 && !allow_smem(reinterpret_cast<const void*>(kv_step_kernel), 3 * sizeof(int) * (kStepMaxRequests + 1), done))
     return B200Q_ERR_CUDA;
   const int grid = grid_for(static_cast<int64_t>(tokens) + requests, 4 * kStepThreads, 1);
   launch_pdl(kv_step_kernel, grid, kStepThreads, smem, static_cast<cudaStream_t>(stream), lens, new_lens, free_pages, nfree,

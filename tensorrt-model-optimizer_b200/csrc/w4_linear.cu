@@ -20,8 +20,6 @@
 // Partial sums meet in shared memory, across the cluster through distributed shared memory, in a fixed order.
 #include <math.h>
 
-#include <atomic>
-
 #include "umma.cuh"
 
 namespace b200q {
@@ -616,8 +614,8 @@ int launch_w4(W4Args a, cudaStream_t s) {
   auto kern = w4_linear_kernel<FMT, T, NT, LW>;
   const int slabs = (a.k + kSlab - 1) / kSlab, sms = sm_count_cached();
   constexpr int kStep = W4Ring<NT>::kSlabs;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kW4SmemLimit)) != cudaSuccess)
-    return B200Q_ERR_CUDA;
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(reinterpret_cast<const void*>(kern), kW4SmemLimit, done)) return B200Q_ERR_CUDA;
   int room = 0;                                     // after the attribute above: the occupancy depends on it
   if (!w4_cut(a.rows, slabs, FMT == kFmtInt4 ? 4 / LW : 0, a.tiles, sms, reinterpret_cast<const void*>(kern), a.wk, a.ks, room))
     return B200Q_ERR_CAPACITY;
