@@ -472,14 +472,17 @@ int b200q_nvfp4_swizzle_scales(const uint8_t* scales, uint8_t* swizzled, int64_t
  *   b200q_nvfp4_linear   W = e2m1 * scales[n, k/16] * (*scale2), codes as b200q_nvfp4_quantize packs them
  * T is B200Q_F16 or B200Q_BF16.  x rows x_stride and out rows out_stride elements apart; x, its stride (in bytes) and
  * codes 16-byte aligned, k a multiple of 32; bias [n] of type T or NULL.  At most 32 rows, and x has to fit on chip:
- * rows up to b200q_w4_linear_max_rows(k) (0: none), more give B200Q_ERR_CAPACITY.  *status_io as in b200q_fp8_gemm. */
+ * rows up to b200q_w4_linear_max_rows(k) (0: none), more give B200Q_ERR_CAPACITY.  workspace:
+ * b200q_w4_linear_workspace(rows, n, k, block) bytes (block 16 for NVFP4; 0 for many shapes: NULL then), this call's
+ * alone until it has run.  *status_io as in b200q_fp8_gemm. */
 int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const void* scales, int block,
                       const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k,
-                      uint32_t* status_io, void* stream);
+                      void* workspace, int64_t workspace_bytes, uint32_t* status_io, void* stream);
 int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales,
                        const float* scale2, const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k,
-                       uint32_t* status_io, void* stream);
+                       void* workspace, int64_t workspace_bytes, uint32_t* status_io, void* stream);
 int b200q_w4_linear_max_rows(int64_t k);
+int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int block);
 
 /* ---------------------------------------------------------------- paged NVFP4 KV cache ------ */
 

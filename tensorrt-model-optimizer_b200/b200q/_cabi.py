@@ -86,15 +86,18 @@ SIGNATURES = {
     "b200q_nvfp4_kv_attention": [_p, _i64, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _i, _i,
                                  _i, _f, _p, _p, _i, _p, _i64, _p],
     "b200q_nvfp4_kv_attention_workspace": [_i, _i, _i, _i, _i],
-    "b200q_int4_linear": [_p, _i64, _i, _p, _p, _i, _p, _p, _i64, _i, _i64, _i64, _p, _p],
-    "b200q_nvfp4_linear": [_p, _i64, _i, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _p, _p],
+    "b200q_int4_linear": [_p, _i64, _i, _p, _p, _i, _p, _p, _i64, _i, _i64, _i64, _p, _i64, _p, _p],
+    "b200q_nvfp4_linear": [_p, _i64, _i, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _p, _i64, _p, _p],
     "b200q_w4_linear_max_rows": [_i64],
+    "b200q_w4_linear_workspace": [_i, _i64, _i64, _i],
     "b200q_mxfp4_quantize": [_p, _i64, _i, _i, _p, _p, _p],
 }
-_RESTYPES = {"b200q_strerror": C.c_char_p, "b200q_nvfp4_kv_attention_workspace": _i64}
+_RESTYPES = {"b200q_strerror": C.c_char_p, "b200q_nvfp4_kv_attention_workspace": _i64,
+             "b200q_w4_linear_workspace": _i64}
 _NO_STATUS = {"b200q_strerror", "b200q_version", "b200q_sm_count", "b200q_nvfp4_group_tile_elems",
               "b200q_nvfp4_group_max_tensors_noalloc", "b200q_qgemm_tile_override",
-              "b200q_nvfp4_kv_attention_workspace", "b200q_w4_linear_max_rows"}
+              "b200q_nvfp4_kv_attention_workspace", "b200q_w4_linear_max_rows",
+              "b200q_w4_linear_workspace"}
 
 
 def _load() -> C.CDLL:

@@ -1112,6 +1112,11 @@ def _w4_max_rows(k: int) -> int:
     return call("b200q_w4_linear_max_rows", k)
 
 
+@functools.lru_cache(maxsize=4096)
+def _w4_workspace(device: int, rows: int, n: int, k: int, block: int) -> int:
+    return call("b200q_w4_linear_workspace", rows, n, k, block)
+
+
 def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, extra, bias):
     _cuda(x, "x"), _cuda(packed, "packed"), _cuda(scales, "scales")
     dev = x.device
@@ -1140,9 +1145,11 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
     most = _w4_max_rows(k)
     with _on(dev):
         for r in range(0, m, most):
+            need = _w4_workspace(dev.index, min(most, m - r), n, k, block)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             call(name, x2.data_ptr() + 2 * r * x2.stride(0), x2.stride(0), _DT[x.dtype], packed.data_ptr(), scales.data_ptr(),
                  extra, bias.data_ptr() if bias is not None else None, out.data_ptr() + 2 * r * n, n, min(most, m - r), n, k,
-                 qgemm_status(dev).data_ptr(), _stream(x))
+                 ws.data_ptr() if need else None, need, qgemm_status(dev).data_ptr(), _stream(x))
     return out
 
 

@@ -14,10 +14,10 @@
 // off by less than 2^-39 of it, far under the 2^-24 of the fp32 sums.  The k order inside a product is free, so a
 // lane's operand is a contiguous run of the packed row and x is put into shared memory in that order.
 //
-// Work.  A cluster of 1 to 8 CTAs shares a tile of 16 weight rows, K split over its CTAs and over their 8 warps,
-// and walks over the row tiles with its part of x resident in shared memory.  Each lane fetches its own operands
-// with cp.async into a ring (kStages x 1 KB a warp, so 96 KB in flight on an SM), which runs on across tiles.
-// Partial sums meet in shared memory, across the cluster through distributed shared memory, in a fixed order.
+// Work.  A CTA of 16 warps has an SM to itself, with its part of x in shared memory: all of K, or one of ks parts
+// where x does not fit (or the tiles are few).  wk of its warps share a tile of 16 weight rows, and it walks over the
+// tiles.  Each warp fetches its codes by TMA into a ring of its own that runs on across tiles (64 to 128 KB on an SM).
+// Sums of the warps meet in shared memory, sums of CTAs in a workspace that a second kernel adds up, in a fixed order.
 #include <math.h>
 
 #include "umma.cuh"
@@ -26,6 +26,7 @@ namespace b200q {
 
 constexpr int kW4Warps = 16, kW4Threads = 32 * kW4Warps;
 constexpr int kW4Rows = 16;                  // weight rows of a tile
+constexpr int kW4MaxParts = 16;              // CTAs that K may be cut over
 constexpr int kSlab = 128;                   // k elements a warp handles at a time
 // Slabs of a step and steps of the ring: four slabs make the bookkeeping of a step cheap; with more than 8 rows
 // shared memory is needed for x and the products themselves take longer, so there two have to do.
@@ -49,6 +50,7 @@ struct W4Args {
   FastDiv pairs;                             // slab pairs of a CTA
   int wide_scales;                           // a lane's scales of a step are one aligned word
   uint32_t* status;
+  float* parts;                              // [ks][rows][n], ks > 1
 };
 
 __device__ __forceinline__ uint32_t w4_pack_f16(float lo, float hi) {
@@ -149,8 +151,7 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   if (threadIdx.x < 8 * NT) xbad[threadIdx.x] = not_finite = 0;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, qd = lane & 3, gr = lane >> 2;
   const int ks = a.ks, wk = a.wk, wr = kW4Warps / wk;
-  const int rank = static_cast<int>(cluster_ctarank());
-  const int cluster = blockIdx.x / ks, nclusters = gridDim.x / ks;
+  const int group = blockIdx.x / ks, groups = gridDim.x / ks, rank = blockIdx.x - group * ks;
   const int slab0 = rank * a.slabs_per_cta;
   const int slabs = max(min(a.slabs_per_cta, (a.k + kSlab - 1) / kSlab - slab0), 0);
   const int my_row = warp / wk, my_k = warp % wk;   // which of the CTA's tiles, which part of its slabs
@@ -159,7 +160,6 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   uint8_t* xs = smem + kW4Warps * kStages * kStageBytes; // [slab][row][i][qd] 16 B
   float* xsum = reinterpret_cast<float*>(xs + static_cast<int64_t>(a.pairs.d) * 2 * kSlab * 2 * a.rows);   // [slab][group][8 NT], INT4
   float* part = xsum + (FMT == kFmtInt4 ? static_cast<int>(a.pairs.d) * 2 * kSegs * 8 * NT : 0);           // [warps][8 NT][16], wk > 1
-  float* recv = part + (wk > 1 ? kW4Warps * kPart : 0);                           // [ks][wr * 16 * rows / ks], ks > 1
   __shared__ __align__(8) uint64_t all_bars[kW4Warps * kStages];
   __shared__ uint32_t abort_flag;
   uint64_t* bars = all_bars + warp * kStages;
@@ -169,11 +169,11 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   __syncthreads();
   pdl_prologue();
 
-  // tiles of round t: (t * wr + my_row) * nclusters + cluster, so that the last round is spread over the SMs
+  // tiles of round t: (t * wr + my_row) * groups + group, so that the last round is spread over the SMs
   const int nsteps = (slabs + kStep - 1) / kStep;
   const int mine = nsteps > my_k ? (nsteps - my_k + wk - 1) / wk : 0;             // steps of this warp in each tile
-  const int first_tile = my_row * nclusters + cluster, tile_step = wr * nclusters;
-  const int rounds = (a.tiles - cluster + tile_step - 1) / tile_step;             // of the CTA
+  const int first_tile = my_row * groups + group, tile_step = wr * groups;
+  const int rounds = (a.tiles - group + tile_step - 1) / tile_step;               // of the CTA
   const int my_tiles = a.tiles > first_tile ? (a.tiles - first_tile + tile_step - 1) / tile_step : 0;
   const int steps = mine * my_tiles;
 
@@ -350,7 +350,7 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   }
 #pragma unroll 1
   for (int u = warp + kHold * kW4Warps; u < units; u += kW4Warps) store_x(u, load_x(u));
-  if (ks > 1) cluster_barrier(); else __syncthreads();   // the others' shared memory may be written from here on
+  __syncthreads();
 
   float back[NT][2];                                // of the columns this thread's sums belong to
   const float s2 = FMT == kFmtNvfp4 ? __ldg(a.scale2) : 16777216.f;                // 2^24 of the codes as subnormals
@@ -366,6 +366,10 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
 
   auto store = [&](int row, int col, float sum) {
     if (col >= a.n) return;
+    if (ks > 1) {                                   // the other parts of K are other CTAs': w4_join_kernel adds them up
+      a.parts[(static_cast<int64_t>(rank) * a.rows + row) * a.n + col] = sum;
+      return;
+    }
     if (a.bias) sum += Elem<T>::to_float(static_cast<const T*>(a.bias)[col]);
     static_cast<T*>(a.out)[row * a.out_stride + col] = Elem<T>::from_float(sum);
   };
@@ -501,14 +505,9 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[n][j] = acc[n][j] * s2 * back[n][j & 1];
 
-    // ---- sums of the K parts, always in the order of the warps and CTAs ----
-    const int elems = kW4Rows * a.rows;             // of a tile
-    const int per = wr * elems / ks;                // of the CTA's tiles that one CTA of the cluster finishes
-    auto push = [&](int e, float v) {               // element e of the CTA's tiles to the CTA that finishes it
-      const uint32_t to = map_to_cta(recv + rank * per + e % per, e / per);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
-    };
+    // ---- sums of the warps' parts of K, always in their order ----
     if (wk > 1) {
+      const int elems = kW4Rows * a.rows;           // of a tile
       float* p = part + warp * kPart;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -519,109 +518,81 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
         const int t = e / elems, in = e - t * elems;
         float sum = 0.f;
         for (int w = 0; w < wk; ++w) sum += part[(t * wk + w) * kPart + in];
-        if (ks > 1) push(e, sum);
-        else store(in / kW4Rows, (first_tile - my_row * nclusters + round * tile_step + t * nclusters) * kW4Rows + in % kW4Rows, sum);
+        store(in / kW4Rows, (group + round * tile_step + t * groups) * kW4Rows + in % kW4Rows, sum);
       }
-      if (ks == 1) __syncthreads();                 // read before the next round writes
-    } else {
+      if (round + 1 < rounds) __syncthreads();      // read before the next round writes
+    } else if (tile < a.tiles) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int wrow = gr + 8 * (j >> 1), row = 8 * n + 2 * qd + (j & 1);
-          if (row >= a.rows) continue;
-          if (ks > 1) push(my_row * elems + row * kW4Rows + wrow, acc[n][j]);
-          else if (tile < a.tiles) store(row, tile * kW4Rows + wrow, acc[n][j]);
+          const int row = 8 * n + 2 * qd + (j & 1);
+          if (row < a.rows) store(row, tile * kW4Rows + gr + 8 * (j >> 1), acc[n][j]);
         }
-    }
-    if (ks > 1) {
-      cluster_barrier();
-      for (int i = threadIdx.x; i < per; i += kW4Threads) {
-        float sum = 0.f;
-        for (int c = 0; c < ks; ++c) sum += recv[c * per + i];
-        const int e = rank * per + i, t = e / elems, in = e - t * elems;
-        store(in / kW4Rows, (cluster + round * tile_step + t * nclusters) * kW4Rows + in % kW4Rows, sum);
-      }
-      if (round + 1 < rounds) cluster_barrier();    // read before the next round's sums arrive
     }
   }
   grace_after_abort(&abort_flag);
 }
 
+// Sums of the CTAs' parts of K, in their order, plus the bias.
+template <typename T>
+__global__ void __launch_bounds__(256) w4_join_kernel(const W4Args a) {
+  pdl_prologue();
+  const int64_t total = static_cast<int64_t>(a.rows) * a.n, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int row = static_cast<int>(i / a.n), col = static_cast<int>(i - static_cast<int64_t>(row) * a.n);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < a.ks; ++p) sum += a.parts[p * total + i];
+  if (a.bias) sum += Elem<T>::to_float(static_cast<const T*>(a.bias)[col]);
+  static_cast<T*>(a.out)[row * a.out_stride + col] = Elem<T>::from_float(sum);
+}
+
 // segs: INT4 groups a slab (0: NVFP4)
-inline size_t w4_smem(int rows, int nt, int slabs, int segs, int wk, int ks) {
+inline size_t w4_smem(int rows, int nt, int slabs, int segs, int wk) {
   const int step = nt == 1 ? W4Ring<1>::kSlabs : W4Ring<2>::kSlabs;
   slabs = (slabs + step - 1) / step * step;
   return kW4Warps * static_cast<size_t>(w4_ring_bytes(nt)) + static_cast<size_t>(slabs) * (kSlab * 2 * rows + 32 * segs * nt) +
-         (wk > 1 ? kW4Warps * kW4Rows * 8 * 4 * static_cast<size_t>(nt) : 0) +
-         (ks > 1 ? static_cast<size_t>(kW4Warps / wk) * kW4Rows * 4 * rows : 0);
+         (wk > 1 ? kW4Warps * kW4Rows * 8 * 4 * static_cast<size_t>(nt) : 0);
 }
 constexpr size_t kW4SmemLimit = 227 * 1024 - 1024;
 inline int w4_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
-// Clusters of `ks` CTAs that run at a time when each fills its SM: a cluster's SMs are of one GPC, so large
-// clusters leave some SMs without work (148 SMs: 74, 33 and 15 clusters of 2, 4 and 8).
-inline int w4_clusters(const void* kern, int ks, int sms) {
-  if (ks == 1) return sms;
-  static std::atomic<int> cached[3];                // clusters of 2, 4, 8
-  std::atomic<int>& slot = cached[ks == 2 ? 0 : ks == 4 ? 1 : 2];
-  int c = slot;
-  if (c == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(sms / ks * ks));
-    cfg.blockDim = dim3(kW4Threads);
-    cfg.dynamicSmemBytes = kW4SmemLimit;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(ks);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) != cudaSuccess || c <= 0) {
-      cudaGetLastError();
-      c = sms / ks;
-    }
-    slot = c;
-  }
-  return c;
-}
-
-// How K is cut over the wk warps of a tile and the ks CTAs of a cluster: the least of an estimate in steps of a
-// fully loaded SM.  A round takes a warp's steps in it; one that leaves warps idle is shorter, but not below what a
-// warp needs by itself (0.6); and each round that joins sums pays for its barriers.
-inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, const void* kern, int& wk, int& ks, int& clusters) {
+// How K is cut, over the wk warps of a tile and over ks CTAs: the least of an estimate in steps of a fully loaded SM.
+// A round takes a warp's steps in it; one that leaves warps idle is shorter, but not below what a warp needs by itself
+// (0.6); a round that joins warps pays for its barriers, and several CTAs for a launch that adds their sums.
+inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, int& wk, int& ks) {
   const int nt = w4_nt(rows), step = nt == 1 ? W4Ring<1>::kSlabs : W4Ring<2>::kSlabs;
   double best = 1e30;
-  for (int c = 1; c <= 8; c *= 2) {
-    const int part = (slabs + c - 1) / c, steps = (part + step - 1) / step;
-    if (c > 1 && part * c / 2 > slabs) break;       // no slab left for the last CTAs
+  for (int c = 1; c <= kW4MaxParts && c <= slabs; ++c) {
+    const int part = ((slabs + c - 1) / c + step - 1) / step * step, steps = part / step;
+    if (c > 1 && part * (c - 1) >= slabs) continue; // nothing left for the last part
     for (int w = 1; w <= kW4Warps && (w == 1 || w <= steps); w *= 2) {
-      if (w4_smem(rows, nt, part, segs, w, c) > kW4SmemLimit) continue;
-      const int held = w4_clusters(kern, c, sms);
-      const double load = static_cast<double>(tiles) * w / (static_cast<double>(held) * kW4Warps);
+      if (w4_smem(rows, nt, part, segs, w) > kW4SmemLimit) continue;
+      const double load = static_cast<double>(tiles) * w / (static_cast<double>(sms / c) * kW4Warps);
       const double whole = floor(load), rest = load - whole;
-      const double rounds = ceil(load), mine = (steps + w - 1) / w;
-      const double cost = mine * (whole + (rest > 0 ? (rest > 0.6 ? rest : 0.6) : 0)) + rounds * ((w > 1 ? 0.15 : 0) + (c > 1 ? 0.4 : 0)) +
-                          (c > 1 ? 0.3 : 0);
-      if (cost < best) { best = cost; wk = w; ks = c; clusters = held; }
+      const double mine = (steps + w - 1) / w;
+      const double cost = mine * (whole + (rest > 0 ? (rest > 0.6 ? rest : 0.6) : 0)) + ceil(load) * (w > 1 ? 0.15 : 0) + (c > 1 ? 2 : 0);
+      if (cost < best) { best = cost; wk = w; ks = c; }
     }
   }
   return best < 1e30;
 }
 
+inline int64_t w4_parts_bytes(int ks, int rows, int64_t n) { return static_cast<int64_t>(ks) * rows * n * 4; }
+
 template <int FMT, typename T, int NT, int LW>
-int launch_w4(W4Args a, cudaStream_t s) {
+int launch_w4(W4Args a, int64_t parts_bytes, cudaStream_t s) {
   auto kern = w4_linear_kernel<FMT, T, NT, LW>;
+  constexpr int kStep = W4Ring<NT>::kSlabs, kGroups = FMT == kFmtInt4 ? 4 / LW : 0;
   const int slabs = (a.k + kSlab - 1) / kSlab, sms = sm_count_cached();
-  constexpr int kStep = W4Ring<NT>::kSlabs;
   static std::atomic<uint64_t> done;
   if (!allow_smem(reinterpret_cast<const void*>(kern), kW4SmemLimit, done)) return B200Q_ERR_CUDA;
-  int room = 0;                                     // after the attribute above: the occupancy depends on it
-  if (!w4_cut(a.rows, slabs, FMT == kFmtInt4 ? 4 / LW : 0, a.tiles, sms, reinterpret_cast<const void*>(kern), a.wk, a.ks, room))
-    return B200Q_ERR_CAPACITY;
+  if (!w4_cut(a.rows, slabs, kGroups, a.tiles, sms, a.wk, a.ks)) return B200Q_ERR_CAPACITY;
+  if (a.ks > 1 && (!a.parts || parts_bytes < w4_parts_bytes(a.ks, a.rows, a.n))) return B200Q_ERR_CAPACITY;
   a.slabs_per_cta = ((slabs + a.ks - 1) / a.ks + kStep - 1) / kStep * kStep;
   a.pairs = FastDiv(a.slabs_per_cta / 2);
-  const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, FMT == kFmtInt4 ? 4 / LW : 0, a.wk, a.ks);
+  const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, kGroups, a.wk);
   const int unit = FMT == kFmtInt4 ? W4Ring<NT>::kSlabs * 4 / LW : 4, bytes = FMT == kFmtInt4 ? 2 : 1;   // scales a lane takes at a time
   a.wide_scales = (FMT == kFmtNvfp4 || LW < 4 || a.group_slabs == 1) && a.groups % unit == 0 &&
                   reinterpret_cast<uintptr_t>(a.scales) % min(unit * bytes, 16) == 0;
@@ -633,31 +604,20 @@ int launch_w4(W4Args a, cudaStream_t s) {
                         CU_TENSOR_MAP_INTERLEAVE_NONE, FMT == kFmtInt4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return B200Q_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kW4Threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(a.ks);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const int clusters = max(1, min(a.tiles, room));
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters * a.ks));
-  cudaLaunchKernelEx(&cfg, kern, map, a);
+  const int groups = max(1, min(a.tiles, sms / a.ks));
+  launch_pdl(kern, groups * a.ks, kW4Threads, smem, s, map, a);
+  if (a.ks > 1)
+    launch_pdl(w4_join_kernel<T>, static_cast<unsigned>((static_cast<int64_t>(a.rows) * a.n + 255) / 256), 256, 0, s, a);
   return launch_status();
 }
 
 template <int FMT, int LW>
-int dispatch_w4(const W4Args& a, int dtype, cudaStream_t s) {
+int dispatch_w4(const W4Args& a, int dtype, int64_t parts_bytes, cudaStream_t s) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (a.rows <= 8) return launch_w4<FMT, T, 1, LW>(a, s);
-    if (a.rows <= 16) return launch_w4<FMT, T, 2, LW>(a, s);
-    return launch_w4<FMT, T, 4, LW>(a, s);
+    if (a.rows <= 8) return launch_w4<FMT, T, 1, LW>(a, parts_bytes, s);
+    if (a.rows <= 16) return launch_w4<FMT, T, 2, LW>(a, parts_bytes, s);
+    return launch_w4<FMT, T, 4, LW>(a, parts_bytes, s);
   };
   return dtype == B200Q_F16 ? go(__half()) : go(__nv_bfloat16());
 }
@@ -675,9 +635,10 @@ inline int w4_check(const void* x, int64_t x_stride, int dtype, const uint8_t* c
 }
 
 inline W4Args w4_args(const void* x, int64_t x_stride, const uint8_t* codes, const void* scales, const float* scale2,
-                      const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, int block, uint32_t* status) {
+                      const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, int block, void* workspace, uint32_t* status) {
   W4Args a{};
   a.status = status;
+  a.parts = static_cast<float*>(workspace);
   a.x = x; a.x_stride = x_stride; a.codes = codes; a.scales = scales; a.scale2 = scale2; a.bias = bias;
   a.out = out; a.out_stride = out_stride;
   a.rows = rows; a.n = static_cast<int>(n); a.k = static_cast<int>(k);
@@ -695,29 +656,40 @@ extern "C" int b200q_w4_linear_max_rows(int64_t k) {
   if (k <= 0 || k % 32 || k > (1 << 24)) return 0;
   const int slabs = static_cast<int>((k + kSlab - 1) / kSlab);
   for (int rows = 32; rows > 0; --rows)
-    if (w4_smem(rows, w4_nt(rows), (slabs + 7) / 8, 4, 1, 8) <= kW4SmemLimit) return rows;
+    if (w4_smem(rows, w4_nt(rows), (slabs + kW4MaxParts - 1) / kW4MaxParts, 4, 1) <= kW4SmemLimit) return rows;
   return 0;
 }
 
+extern "C" int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int block) {
+  if (rows <= 0 || rows > 32 || n <= 0 || n > (1 << 30) || k <= 0 || k % 32 || k > (1 << 24) || block <= 0) return B200Q_ERR_SHAPE;
+  int wk = 1, ks = 1;
+  const int groups = block == 16 ? 0 : block == 32 ? 4 : block == 64 ? 2 : 1;
+  if (!w4_cut(rows, static_cast<int>((k + kSlab - 1) / kSlab), groups, static_cast<int>((n + kW4Rows - 1) / kW4Rows), sm_count_cached(), wk, ks))
+    return B200Q_ERR_CAPACITY;
+  return ks > 1 ? w4_parts_bytes(ks, rows, n) : 0;
+}
+
 extern "C" int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const void* scales, int block,
-                                 const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, uint32_t* status_io, void* stream) {
+                                 const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                                 uint32_t* status_io, void* stream) {
   B200Q_REQUIRE_PTR(status_io);
   if (const int r = w4_check(x, x_stride, dtype, codes, scales, out, out_stride, rows, n, k)) return r;
   if (block <= 0 || k % block) return B200Q_ERR_SHAPE;
   if (block != 32 && block != 64 && block % kSlab) return B200Q_ERR_UNSUPPORTED;
-  const W4Args a = w4_args(x, x_stride, codes, scales, nullptr, bias, out, out_stride, rows, n, k, block, status_io);
+  const W4Args a = w4_args(x, x_stride, codes, scales, nullptr, bias, out, out_stride, rows, n, k, block, workspace, status_io);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (block == 32) return dispatch_w4<kFmtInt4, 1>(a, dtype, s);
-  if (block == 64) return dispatch_w4<kFmtInt4, 2>(a, dtype, s);
-  return dispatch_w4<kFmtInt4, 4>(a, dtype, s);
+  if (block == 32) return dispatch_w4<kFmtInt4, 1>(a, dtype, workspace_bytes, s);
+  if (block == 64) return dispatch_w4<kFmtInt4, 2>(a, dtype, workspace_bytes, s);
+  return dispatch_w4<kFmtInt4, 4>(a, dtype, workspace_bytes, s);
 }
 
 extern "C" int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales,
                                   const float* scale2, const void* bias, void* out, int64_t out_stride, int rows, int64_t n,
-                                  int64_t k, uint32_t* status_io, void* stream) {
+                                  int64_t k, void* workspace, int64_t workspace_bytes,
+                                 uint32_t* status_io, void* stream) {
   B200Q_REQUIRE_PTR(status_io);
   if (const int r = w4_check(x, x_stride, dtype, codes, scales, out, out_stride, rows, n, k)) return r;
   B200Q_REQUIRE_PTR(scale2);
-  const W4Args a = w4_args(x, x_stride, codes, scales, scale2, bias, out, out_stride, rows, n, k, 16, status_io);
-  return dispatch_w4<kFmtNvfp4, 4>(a, dtype, static_cast<cudaStream_t>(stream));
+  const W4Args a = w4_args(x, x_stride, codes, scales, scale2, bias, out, out_stride, rows, n, k, 16, workspace, status_io);
+  return dispatch_w4<kFmtNvfp4, 4>(a, dtype, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
