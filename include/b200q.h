@@ -469,20 +469,22 @@ int b200q_nvfp4_swizzle_scales(const uint8_t* scales, uint8_t* swizzled, int64_t
  * never dequantised to memory; fp32 sums, one rounding.
  *   b200q_int4_linear    W = (code - 8) / scales[n, k/block], codes as b200q_int4_quantize packs them (even element
  *                        in the high nibble), scales of type T; block 32, 64 or a multiple of 128 that divides k
- *   b200q_nvfp4_linear   W = e2m1 * scales[n, k/16] * (*scale2), codes as b200q_nvfp4_quantize packs them
+ *   b200q_nvfp4_linear   W = e2m1 * scales[n, k/block] * (*scale2), codes as b200q_nvfp4_quantize(_blocks)
+ *                        packs them; block 16 or 32
  * T is B200Q_F16 or B200Q_BF16.  x rows x_stride and out rows out_stride elements apart; x, its stride (in bytes) and
  * codes 16-byte aligned, k a multiple of 32; bias [n] of type T or NULL.  At most 32 rows, and x has to fit on chip:
  * rows up to b200q_w4_linear_max_rows(k) (0: none), more give B200Q_ERR_CAPACITY.  workspace:
- * b200q_w4_linear_workspace(rows, n, k, block) bytes (block 16 for NVFP4; 0 for many shapes: NULL then), this call's
+ * b200q_w4_linear_workspace(rows, n, k, int4_block) bytes (int4_block 0 for NVFP4; the answer is 0 for many shapes:
+ * NULL then), this call's
  * alone until it has run.  *status_io as in b200q_fp8_gemm. */
 int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const void* scales, int block,
                       const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k,
                       void* workspace, int64_t workspace_bytes, uint32_t* status_io, void* stream);
-int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales,
+int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales, int block,
                        const float* scale2, const void* bias, void* out, int64_t out_stride, int rows, int64_t n, int64_t k,
                        void* workspace, int64_t workspace_bytes, uint32_t* status_io, void* stream);
 int b200q_w4_linear_max_rows(int64_t k);
-int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int block);
+int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int int4_block);
 
 /* ---------------------------------------------------------------- paged NVFP4 KV cache ------ */
 

@@ -87,7 +87,7 @@ SIGNATURES = {
                                  _i, _f, _p, _p, _i, _p, _i64, _p],
     "b200q_nvfp4_kv_attention_workspace": [_i, _i, _i, _i, _i],
     "b200q_int4_linear": [_p, _i64, _i, _p, _p, _i, _p, _p, _i64, _i, _i64, _i64, _p, _i64, _p, _p],
-    "b200q_nvfp4_linear": [_p, _i64, _i, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _p, _i64, _p, _p],
+    "b200q_nvfp4_linear": [_p, _i64, _i, _p, _p, _i, _p, _p, _p, _i64, _i, _i64, _i64, _p, _i64, _p, _p],
     "b200q_w4_linear_max_rows": [_i64],
     "b200q_w4_linear_workspace": [_i, _i64, _i64, _i],
     "b200q_mxfp4_quantize": [_p, _i64, _i, _i, _p, _p, _p],

@@ -46,11 +46,17 @@ def _both_quantizers_enabled(module) -> bool:
     return bool(iq is not None and wq is not None and iq.is_enabled and wq.is_enabled)
 
 
-def enable_real_quant_gemm(model: nn.Module) -> None:
+def _only_weight_quantizer_enabled(module) -> bool:
+    iq, wq = getattr(module, "input_quantizer", None), getattr(module, "weight_quantizer", None)
+    return bool(iq is not None and wq is not None and not iq.is_enabled and wq.is_enabled)
+
+
+def enable_real_quant_gemm(model: nn.Module, weight_only: bool = False) -> None:
     """Mark every module whose input and weight quantisers are both enabled to use a registered
-    real-quant GEMM."""
+    real-quant GEMM.  ``weight_only`` marks those too whose weight quantiser alone is enabled: with a packed
+    4-bit weight and few rows they then read the packed weight instead of dequantising it first."""
     for module in model.modules():
-        if _both_quantizers_enabled(module):
+        if _both_quantizers_enabled(module) or (weight_only and _only_weight_quantizer_enabled(module)):
             module._use_real_quant_gemm = True
 
 

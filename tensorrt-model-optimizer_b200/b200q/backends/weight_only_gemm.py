@@ -1,0 +1,95 @@
+"""Linear layers with packed 4-bit weights and 16-bit activations for decoding batches.
+
+A weight-only layer (``INT4_AWQ_CFG``, ``INT4_BLOCKWISE_WEIGHT_ONLY_CFG``, ``NVFP4_MLP_WEIGHT_ONLY_CFG`` after
+``compress``) dequantises its whole weight to memory in every forward pass.  For a few rows the products of
+``ops.int4_linear`` / ``ops.nvfp4_linear`` read the packed weight once instead.  They keep the sums in fp32 and do not
+round the dequantised weight to 16 bits, so results differ from the dequantising path in the last bits; layers use them
+after ``enable_real_quant_gemm(model, weight_only=True)`` (or ``compress(model, {"weight_only_gemm": True})``)."""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch.autograd import Function
+
+from .. import ops
+from ..qtensor import INT4QTensor, NVFP4QTensor, QTensorWrapper
+from .gemm_registry import gemm_registry
+
+__all__ = ["WeightOnlyLinear", "weight_only_gemm", "WEIGHT_ONLY_MAX_ROWS"]
+
+# Rows up to which the packed weight is used; more go through the dequantised weight and a library GEMM.  Measured on
+# 4096 x 4096, 8192 x 8192, 8192 x 28672 and 28672 x 8192 weights (us, packed against dequantised): INT4 at 128 rows
+# 46 / 52, 111 / 226, 272 / 783, 307 / 796 (at 256 rows 92 / 53 on the smallest); NVFP4 at 32 rows 11 / 14, 25 / 53,
+# 60 / 182, 68 / 187 (at 64 rows 21 / 14 on the smallest).
+WEIGHT_ONLY_MAX_ROWS = {INT4QTensor: 128, NVFP4QTensor: 32}
+
+
+def weight_only_gemm(quant_module, input_tensor, bias=None):
+    """``input [..., k]`` times the module's packed 4-bit weight ``[n, k]``."""
+    wq, weight = quant_module.weight_quantizer, quant_module.weight
+    n, k = weight.metadata["shape"]
+    packed = weight.data.reshape(n, k // 2)
+    block = wq.block_sizes[-1]
+    if weight.metadata["qtensor_class"] is INT4QTensor:
+        return ops.int4_linear(input_tensor, packed, wq._scale, block, bias)
+    return ops.nvfp4_linear(input_tensor, packed, wq._scale, wq._double_scale, bias, block)
+
+
+def _covered(module, input) -> bool:
+    """Whether the module's weight is packed in a layout that the products read, for inputs like ``input``."""
+    wq, weight = module.weight_quantizer, module.weight
+    if not isinstance(weight, QTensorWrapper) or not weight.data.is_cuda or not hasattr(wq, "_scale"):
+        return False
+    kind, shape, dtype = (weight.metadata[key] for key in ("qtensor_class", "shape", "dtype"))
+    if kind not in (INT4QTensor, NVFP4QTensor) or len(shape) != 2 or dtype != input.dtype or input.shape[-1] != shape[1]:
+        return False
+    block = (getattr(wq, "block_sizes", None) or {}).get(-1)
+    if not isinstance(block, int) or weight.data.numel() * 2 != shape[0] * shape[1]:      # padded rows
+        return False
+    if kind is INT4QTensor:
+        return wq._scale.dtype == input.dtype and ops.int4_linear_supported(input, shape[1], block)
+    return hasattr(wq, "_double_scale") and ops.nvfp4_linear_supported(input, shape[1], block)
+
+
+def _weight_only_availability_check(module, input, args, kwargs) -> bool:
+    from ..nn import RealQuantLinear, TensorQuantizer
+
+    if not (isinstance(module, RealQuantLinear) and isinstance(getattr(module, "input_quantizer", None), TensorQuantizer)
+            and isinstance(getattr(module, "weight_quantizer", None), TensorQuantizer)):
+        return False
+    return (not module.input_quantizer.is_enabled and module.weight_quantizer.is_enabled and torch.cuda.is_available()
+            and input.is_cuda and _covered(module, input))
+
+
+class WeightOnlyLinear(Function):
+    """Autograd wrapper: forward on the packed weight, the input's gradient through the dequantised weight (the
+    packed weight itself is not trained)."""
+
+    @staticmethod
+    def forward(ctx, quant_module, input_tensor, weight, bias=None):
+        ctx.quant_module = quant_module
+        ctx.save_for_backward(weight)
+        ctx.bias_grad = bias is not None and bias.requires_grad
+        return weight_only_gemm(quant_module, input_tensor, bias)
+
+    @staticmethod
+    def backward(ctx, grad_outputs):
+        weight, = ctx.saved_tensors
+        grad_input = grad_bias = None
+        if ctx.needs_input_grad[1]:
+            grad_input = grad_outputs @ ctx.quant_module.weight_quantizer.dequantize(weight)
+        if ctx.bias_grad:
+            grad_bias = grad_outputs.sum(dim=list(range(grad_outputs.dim() - 1)))
+        return None, grad_input, None, grad_bias
+
+
+def _weight_only_linear(quant_module, input, weight, bias=None):
+    x = quant_module.input_quantizer(input)               # a disabled quantiser still applies its AWQ pre-quant scale
+    if not _covered(quant_module, x) or x.numel() // x.shape[-1] > WEIGHT_ONLY_MAX_ROWS[weight.metadata["qtensor_class"]]:
+        return F.linear(x, quant_module._quantized_weight(), bias)
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        return WeightOnlyLinear.apply(quant_module, x, weight, bias)
+    return weight_only_gemm(quant_module, x, bias)
+
+
+gemm_registry.register(gemm_func=_weight_only_linear, availability_check=_weight_only_availability_check)

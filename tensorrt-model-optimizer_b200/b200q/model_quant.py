@@ -74,9 +74,9 @@ def compress(model: nn.Module, config=None) -> nn.Module:
 
     ``config`` may carry ``{"compress": {pattern: bool}}`` to choose layers by name and
     ``{"quant_gemm": bool}`` (default on, as in the reference's compress.py:124-128): layers whose input and
-    weight quantisers are both enabled are marked to run a registered real-quantisation GEMM."""
-    from .backends.gemm_registry import disable_real_quant_gemm, enable_real_quant_gemm
-
+    weight quantisers are both enabled are marked to run a registered real-quantisation GEMM.
+    ``{"weight_only_gemm": bool}`` (default off): layers whose weight quantiser alone is enabled are marked too
+    (``backends.enable_real_quant_gemm(model, weight_only=True)``)."""
     patterns = (config or {}).get("compress", {"default": True}) if isinstance(config, dict) else {"default": True}
     with SequentialQuantizer.convert_to_single_quantizer(model):
         for name, m in model.named_modules():
@@ -94,9 +94,22 @@ def compress(model: nn.Module, config=None) -> nn.Module:
             wq._dequantize = False
         pack_real_quantize_weight(model)
     quant_gemm = bool(config.get("quant_gemm", True)) if isinstance(config, dict) else True
-    (enable_real_quant_gemm if quant_gemm else disable_real_quant_gemm)(model)
-    _record_mode(model, "real_quantize", {"quant_gemm": quant_gemm})
+    weight_only = bool(config.get("weight_only_gemm", False)) if isinstance(config, dict) else False
+    _set_real_quant_gemm(model, quant_gemm, weight_only)
+    record = {"quant_gemm": quant_gemm}
+    if weight_only:
+        record["weight_only_gemm"] = True
+    _record_mode(model, "real_quantize", record)
     return model
+
+
+def _set_real_quant_gemm(model: nn.Module, quant_gemm: bool, weight_only: bool):
+    from .backends.gemm_registry import disable_real_quant_gemm, enable_real_quant_gemm
+
+    if quant_gemm:
+        enable_real_quant_gemm(model, weight_only=weight_only)
+    else:
+        disable_real_quant_gemm(model)
 
 
 def postprocess_amax(model: nn.Module, key: str, post_process_fn) -> nn.Module:
@@ -197,7 +210,6 @@ def restore_from_modelopt_state(model: nn.Module, state: dict) -> nn.Module:
         m.weight = QTensorWrapper(packed, metadata=dict(meta["metadata"]))
     for mode, cfg in modes:
         if mode == "real_quantize":
-            from .backends.gemm_registry import disable_real_quant_gemm, enable_real_quant_gemm
-            (enable_real_quant_gemm if (cfg or {}).get("quant_gemm", True) else disable_real_quant_gemm)(model)
+            _set_real_quant_gemm(model, (cfg or {}).get("quant_gemm", True), (cfg or {}).get("weight_only_gemm", False))
     model.__dict__["_b200q_state"] = list(modes)
     return model

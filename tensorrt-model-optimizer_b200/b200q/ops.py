@@ -1100,24 +1100,33 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
 
 # --------------------------------------------------------------------------- few rows, 4-bit weights --
 
-def w4_linear_supported(x: torch.Tensor, k: int, block: int) -> bool:
-    """Whether ``int4_linear`` (``block`` its group) / ``nvfp4_linear`` (block 16) cover x [..., k]."""
+def int4_linear_supported(x: torch.Tensor, k: int, block: int) -> bool:
+    """Whether ``int4_linear`` covers x [..., k] with groups of ``block``."""
+    return _w4_covers(x, k, block) and (block in (32, 64) or block % 128 == 0)
+
+
+def nvfp4_linear_supported(x: torch.Tensor, k: int, block: int = 16) -> bool:
+    """Whether ``nvfp4_linear`` covers x [..., k] with scale blocks of ``block``."""
+    return _w4_covers(x, k, block) and block in (16, 32)
+
+
+def _w4_covers(x: torch.Tensor, k: int, block: int) -> bool:
     return (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1 and x.shape[-1] == k
-            and k % 32 == 0 and block > 0 and k % block == 0 and (block in (16, 32, 64) or block % 128 == 0)
-            and _w4_max_rows(k) > 0)
+            and k % 32 == 0 and block > 0 and k % block == 0 and _w4_max_rows(k) > 0)
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=4096)
 def _w4_max_rows(k: int) -> int:
     return call("b200q_w4_linear_max_rows", k)
 
 
 @functools.lru_cache(maxsize=4096)
-def _w4_workspace(device: int, rows: int, n: int, k: int, block: int) -> int:
-    return call("b200q_w4_linear_workspace", rows, n, k, block)
+def _w4_workspace(device: int, rows: int, n: int, k: int, int4_block: int) -> int:
+    return call("b200q_w4_linear_workspace", rows, n, k, int4_block)
 
 
-def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, extra, bias):
+def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, covers, int4_block: int,
+               scale2, bias):
     _cuda(x, "x"), _cuda(packed, "packed"), _cuda(scales, "scales")
     dev = x.device
     if x.dtype not in (torch.float16, torch.bfloat16):
@@ -1125,13 +1134,12 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
     if packed.dim() != 2 or packed.element_size() != 1:
         raise ValueError("b200q: packed must be [n, k/2] bytes")
     n, k = packed.shape[0], 2 * packed.shape[1]
-    if n == 0 or not w4_linear_supported(x, k, block):
+    if n == 0 or not covers(x, k, block):
         raise ValueError(f"b200q: no 4-bit product for x {tuple(x.shape)}, weight [{n}, {k}], block {block}")
     if scales.numel() != n * (k // block):
         raise ValueError(f"b200q: expected {n * (k // block)} scales, got {scales.numel()}")
-    for t in (packed, scales) if bias is None else (packed, scales, bias):
-        if t.device != dev:
-            raise ValueError("b200q: x, weight and bias must be on one device")
+    if packed.device != dev or scales.device != dev or (bias is not None and bias.device != dev):
+        raise ValueError("b200q: x, weight and bias must be on one device")
     if bias is not None:
         if bias.numel() != n:
             raise ValueError(f"b200q: bias must have {n} elements")
@@ -1140,39 +1148,39 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     if x2.stride(1) != 1 or (x2.data_ptr() | 2 * x2.stride(0)) & 15:
         x2 = x2.clone(memory_format=torch.contiguous_format)
-    m = x2.shape[0]
+    m, xs = x2.shape[0], x2.stride(0)
     out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
-    most = _w4_max_rows(k)
+    most, bias_at = _w4_max_rows(k), bias.data_ptr() if bias is not None else None
+    extra = (block,) if scale2 is None else (block, scale2.data_ptr())
     with _on(dev):
         for r in range(0, m, most):
-            need = _w4_workspace(dev.index, min(most, m - r), n, k, block)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            call(name, x2.data_ptr() + 2 * r * x2.stride(0), x2.stride(0), _DT[x.dtype], packed.data_ptr(), scales.data_ptr(),
-                 extra, bias.data_ptr() if bias is not None else None, out.data_ptr() + 2 * r * n, n, min(most, m - r), n, k,
-                 ws.data_ptr() if need else None, need, qgemm_status(dev).data_ptr(), _stream(x))
+            rows = min(most, m - r)
+            need = _w4_workspace(dev.index, rows, n, k, int4_block)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None    # this call's own
+            call(name, x2.data_ptr() + 2 * r * xs, xs, _DT[x.dtype], packed.data_ptr(), scales.data_ptr(), *extra, bias_at,
+                 out.data_ptr() + 2 * r * n, n, rows, n, k, ws.data_ptr() if need else None, need,
+                 qgemm_status(dev).data_ptr(), _stream(x))
     return out
 
 
 def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, bias: torch.Tensor | None = None):
     """x [..., k] times an INT4 weight -> [..., n] in x's dtype: W = (code - 8) / scale, ``packed`` uint8 [n, k/2] (even
     element in the high nibble) and ``scales`` [n * k/block, 1] in x's dtype as ``int4_quantize`` gives them for a
-    weight whose rows are whole blocks.  float16 / bfloat16; block 32, 64 or a multiple of 128.  The weight is read
-    once for every 32 rows (fewer where k is very long), without being dequantised to memory: for decoding batches; a
-    long prompt is faster through ``int4_dequantize`` and a GEMM."""
+    weight whose rows are whole blocks.  float16 / bfloat16; block 32, 64 or a multiple of 128; k a multiple of 32.  The
+    weight is read once for every 32 rows (fewer where k is very long) and never dequantised to memory: for decoding
+    batches; a long prompt is faster through ``int4_dequantize`` and a GEMM."""
     if scales.dtype != x.dtype:
         raise TypeError(f"b200q: int4_linear takes scales of x's dtype {x.dtype}, got {scales.dtype}")
-    if block == 16:
-        raise ValueError("b200q: int4_linear covers groups of 32, 64 and multiples of 128")
-    return _w4_linear("b200q_int4_linear", x, packed, scales, block, block, bias)
+    return _w4_linear("b200q_int4_linear", x, packed, scales, block, int4_linear_supported, block, None, bias)
 
 
 def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, scale2: torch.Tensor,
-                 bias: torch.Tensor | None = None):
+                 bias: torch.Tensor | None = None, block: int = 16):
     """x [..., k] times an NVFP4 weight, x left in 16 bits -> [..., n] in x's dtype: W = e2m1 * scale * scale2 with
-    ``packed`` uint8 [n, k/2], ``scales`` float8_e4m3fn [n, k/16] and ``scale2`` fp32 as ``nvfp4_quantize`` gives them.
-    Like ``int4_linear`` in everything else."""
+    ``packed`` uint8 [n, k/2], ``scales`` float8_e4m3fn [n, k/block] and ``scale2`` fp32 as ``nvfp4_quantize`` gives
+    them; block 16 or 32.  Like ``int4_linear`` in everything else."""
     if scales.element_size() != 1:
         raise TypeError("b200q: nvfp4_linear takes float8_e4m3fn scales")
     _cuda(x, "x")
     s2 = _kv_scale2(scale2, x.device)
-    return _w4_linear("b200q_nvfp4_linear", x, packed, scales, 16, s2.data_ptr(), bias)
+    return _w4_linear("b200q_nvfp4_linear", x, packed, scales, block, nvfp4_linear_supported, 0, s2, bias)

@@ -1,6 +1,7 @@
 // Products of a few rows with 4-bit weights:  out[m, n] = T(sum_k x[m, k] W[n, k] + bias[n])  with
 //   INT4   W = (code - 8) / scale, one scale of type T per row and group (INT4QTensor; even element in the high nibble)
-//   NVFP4  W = e2m1 * e4m3 * scale2, one E4M3 scale per row and 16 elements (NVFP4QTensor; even element in the low nibble)
+//   NVFP4  W = e2m1 * e4m3 * scale2, one E4M3 scale per row and 16 or 32 elements (NVFP4QTensor; even element in the low
+//          nibble)
 // The weight is read once, in the layout it is stored in; nothing is dequantised to memory.
 //
 // What bounds it: 0.52 / 0.56 bytes a weight from HBM.  At the measured copy rate an SM gets 46 weights a clock,
@@ -40,7 +41,7 @@ struct W4Args {
   const void* x;
   int64_t x_stride;                          // elements
   const uint8_t* codes;                      // [n, k/2]
-  const void* scales;                        // INT4: T [n, k/block]; NVFP4: E4M3 [n, k/16]
+  const void* scales;                        // INT4: T [n, k/block]; NVFP4: E4M3 [n, k/block]
   const float* scale2;                       // NVFP4
   const void* bias;                          // T [n] or NULL
   void* out;                                 // [rows, n]
@@ -132,7 +133,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-enum { kFmtInt4 = 0, kFmtNvfp4 = 1 };
+enum { kFmtInt4 = 0, kFmtNvfp4 = 1, kFmtNvfp4x32 = 2 };   // x32: one E4M3 scale for 32 elements
 
 // LW: words (of 8 codes) in a lane's contiguous run.  Lane qd of a quad holds the elements
 //   slab * 128 + (i / LW) * 32 LW + qd * 8 LW + 8 (i % LW) + 0..7   for i = 0..3,
@@ -213,7 +214,7 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
         for (int r = 0; r < 2; ++r)
           ps[r] = static_cast<const uint8_t*>(a.scales) +
                   static_cast<int64_t>(min(s_tile * kW4Rows + gr + 8 * r, a.n - 1)) * a.groups * (FMT == kFmtInt4 ? 2 : 1);
-        s_at = FMT == kFmtInt4 ? slab_first * kSegs : slab_first * (kSlab / 16) + 4 * qd;
+        s_at = FMT == kFmtInt4 ? slab_first * kSegs : FMT == kFmtNvfp4 ? slab_first * (kSlab / 16) + 4 * qd : slab_first * (kSlab / 32) + 2 * qd;
         s_tile += tile_step;
       }
       if constexpr (FMT == kFmtInt4) {
@@ -241,9 +242,12 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
           for (int w = 0; w < kPairs; ++w) {
-            const int at = s_at + 16 * w;
+            const int at = s_at + (FMT == kFmtNvfp4 ? 16 : 8) * w;
             nxt[r][w] = 0;
-            if (a.wide_scales) {
+            if constexpr (FMT == kFmtNvfp4x32) {    // the scales of the lane's two runs of 32
+              if (at < a.groups) nxt[r][w] = __ldg(ps[r] + at);
+              if (at + 1 < a.groups) nxt[r][w] |= static_cast<uint32_t>(__ldg(ps[r] + at + 1)) << 8;
+            } else if (a.wide_scales) {
               if (at < a.groups) nxt[r][w] = __ldg(reinterpret_cast<const uint32_t*>(ps[r] + at));
             } else {
               if (at < a.groups) nxt[r][w] = __ldg(reinterpret_cast<const uint16_t*>(ps[r] + at));
@@ -252,7 +256,7 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
           }
         }
       }
-      s_at += FMT == kFmtInt4 ? kStep * wk * kSegs : kStep * wk * (kSlab / 16);
+      s_at += FMT == kFmtInt4 ? kStep * wk * kSegs : kStep * wk * (kSlab / (FMT == kFmtNvfp4 ? 16 : 32));
       if (++s_i == mine) s_i = 0;
       --s_left;
     }
@@ -353,7 +357,7 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   __syncthreads();
 
   float back[NT][2];                                // of the columns this thread's sums belong to
-  const float s2 = FMT == kFmtNvfp4 ? __ldg(a.scale2) : 16777216.f;                // 2^24 of the codes as subnormals
+  const float s2 = FMT != kFmtInt4 ? __ldg(a.scale2) : 16777216.f;                // 2^24 of the codes as subnormals
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -407,7 +411,7 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
       for (int j4 = 0; j4 < kStep; ++j4) {          // behind the end of K x is zero
         const int half = j4 & 1;
         uint32_t wa[4], wb[4];
-        if constexpr (FMT == kFmtNvfp4) {           // 128-byte rows, 16-byte pieces swizzled by the row
+        if constexpr (FMT != kFmtInt4) {            // 128-byte rows, 16-byte pieces swizzled by the row
           const uint8_t* p = ring + slot + (j4 / 2) * 2048 + gr * 128 + (((2 * qd + half) ^ gr) << 4);
           const uint4 va = *reinterpret_cast<const uint4*>(p), vb = *reinterpret_cast<const uint4*>(p + 1024);
           wa[0] = va.x; wa[1] = va.y; wa[2] = va.z; wa[3] = va.w;
@@ -421,13 +425,14 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
           }
         }
         uint32_t sc[2][2];
-        if constexpr (FMT == kFmtNvfp4) {
+        if constexpr (FMT != kFmtInt4) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             uint32_t h;
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(cur[r][j4 / 2] >> (16 * half))));
-            sc[r][0] = __byte_perm(h, h, 0x1010);
-            sc[r][1] = __byte_perm(h, h, 0x3232);
+            const uint32_t two = FMT == kFmtNvfp4 ? cur[r][j4 / 2] >> (16 * half) : cur[r][j4 / 2];
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+            sc[r][0] = __byte_perm(h, h, FMT == kFmtNvfp4 || half == 0 ? 0x1010 : 0x3232);
+            sc[r][1] = __byte_perm(h, h, FMT == kFmtNvfp4 || half == 1 ? 0x3232 : 0x1010);
           }
         }
         float tmp[NT][4], stmp[NT][4];
@@ -594,7 +599,7 @@ int launch_w4(W4Args a, int64_t parts_bytes, cudaStream_t s) {
   a.pairs = FastDiv(a.slabs_per_cta / 2);
   const size_t smem = w4_smem(a.rows, NT, a.slabs_per_cta, kGroups, a.wk);
   const int unit = FMT == kFmtInt4 ? W4Ring<NT>::kSlabs * 4 / LW : 4, bytes = FMT == kFmtInt4 ? 2 : 1;   // scales a lane takes at a time
-  a.wide_scales = (FMT == kFmtNvfp4 || LW < 4 || a.group_slabs == 1) && a.groups % unit == 0 &&
+  a.wide_scales = (FMT != kFmtInt4 || LW < 4 || a.group_slabs == 1) && a.groups % unit == 0 &&
                   reinterpret_cast<uintptr_t>(a.scales) % min(unit * bytes, 16) == 0;
   CUtensorMap map;
   const EncodeTiledFn encode = encode_tiled_fn();
@@ -660,10 +665,10 @@ extern "C" int b200q_w4_linear_max_rows(int64_t k) {
   return 0;
 }
 
-extern "C" int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int block) {
-  if (rows <= 0 || rows > 32 || n <= 0 || n > (1 << 30) || k <= 0 || k % 32 || k > (1 << 24) || block <= 0) return B200Q_ERR_SHAPE;
+extern "C" int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int int4_block) {
+  if (rows <= 0 || rows > 32 || n <= 0 || n > (1 << 30) || k <= 0 || k % 32 || k > (1 << 24) || int4_block < 0) return B200Q_ERR_SHAPE;
   int wk = 1, ks = 1;
-  const int groups = block == 16 ? 0 : block == 32 ? 4 : block == 64 ? 2 : 1;
+  const int groups = int4_block == 0 ? 0 : int4_block == 32 ? 4 : int4_block == 64 ? 2 : 1;
   if (!w4_cut(rows, static_cast<int>((k + kSlab - 1) / kSlab), groups, static_cast<int>((n + kW4Rows - 1) / kW4Rows), sm_count_cached(), wk, ks))
     return B200Q_ERR_CAPACITY;
   return ks > 1 ? w4_parts_bytes(ks, rows, n) : 0;
@@ -683,13 +688,15 @@ extern "C" int b200q_int4_linear(const void* x, int64_t x_stride, int dtype, con
   return dispatch_w4<kFmtInt4, 4>(a, dtype, workspace_bytes, s);
 }
 
-extern "C" int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales,
+extern "C" int b200q_nvfp4_linear(const void* x, int64_t x_stride, int dtype, const uint8_t* codes, const uint8_t* scales, int block,
                                   const float* scale2, const void* bias, void* out, int64_t out_stride, int rows, int64_t n,
                                   int64_t k, void* workspace, int64_t workspace_bytes,
                                  uint32_t* status_io, void* stream) {
   B200Q_REQUIRE_PTR(status_io);
   if (const int r = w4_check(x, x_stride, dtype, codes, scales, out, out_stride, rows, n, k)) return r;
   B200Q_REQUIRE_PTR(scale2);
-  const W4Args a = w4_args(x, x_stride, codes, scales, scale2, bias, out, out_stride, rows, n, k, 16, workspace, status_io);
-  return dispatch_w4<kFmtNvfp4, 4>(a, dtype, workspace_bytes, static_cast<cudaStream_t>(stream));
+  if (block != 16 && block != 32) return B200Q_ERR_UNSUPPORTED;
+  const W4Args a = w4_args(x, x_stride, codes, scales, scale2, bias, out, out_stride, rows, n, k, block, workspace, status_io);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return block == 16 ? dispatch_w4<kFmtNvfp4, 4>(a, dtype, workspace_bytes, s) : dispatch_w4<kFmtNvfp4x32, 4>(a, dtype, workspace_bytes, s);
 }

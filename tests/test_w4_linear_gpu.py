@@ -21,15 +21,15 @@ def _int4(n, k, block, dtype, seed):
     return packed, scales, ((c - 8) / scales.reshape(n, -1, 1).double()).reshape(n, k)
 
 
-def _nvfp4(n, k, dtype, seed):
+def _nvfp4(n, k, dtype, seed, block=16):
     from b200q import ops
 
     g = torch.Generator(device=DEV).manual_seed(seed)
     w = (torch.randn(n, k, generator=g, device=DEV) * torch.logspace(-3, 0, n, device=DEV).unsqueeze(1)).to(dtype)
-    packed, scales, s2 = ops.nvfp4_quantize(w)
+    packed, scales, s2 = ops.nvfp4_quantize(w, block=block)
     lut = torch.tensor(E2M1, dtype=torch.float64, device=DEV)
     v = lut[torch.stack((packed & 15, packed >> 4), -1).reshape(n, k).long()]
-    return packed, scales, s2, (v.reshape(n, -1, 16) * scales.float().double().unsqueeze(-1)).reshape(n, k) * s2.double()
+    return packed, scales, s2, (v.reshape(n, -1, block) * scales.float().double().unsqueeze(-1)).reshape(n, k) * s2.double()
 
 
 def _close(out, x, w, bias=None):
@@ -67,6 +67,16 @@ def test_nvfp4_linear(dtype, m, n, k):
     packed, scales, s2, w = _nvfp4(n, k, dtype, seed=n + m)
     x = _x(m, k, dtype, m)
     _close(ops.nvfp4_linear(x, packed, scales, s2), x, w)
+
+
+@pytest.mark.parametrize("m", [1, 5, 12, 32])
+@pytest.mark.parametrize("n,k", [(1, 32), (20, 96), (17, 288), (100, 4096), (16, 8224)])
+def test_nvfp4_linear_with_scale_blocks_of_32(m, n, k):
+    from b200q import ops
+
+    packed, scales, s2, w = _nvfp4(n, k, torch.bfloat16, seed=n + m, block=32)
+    x = _x(m, k, torch.bfloat16, m)
+    _close(ops.nvfp4_linear(x, packed, scales, s2, block=32), x, w)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -206,4 +216,7 @@ def test_refusals():
         ops.int4_linear(x.cpu(), packed, scales, 128)
     with pytest.raises(TypeError):
         ops.nvfp4_linear(x, packed, scales, torch.ones((), device=DEV))
-    assert not ops.w4_linear_supported(x[:, :16], 16, 16)
+    with pytest.raises(ValueError):
+        ops.nvfp4_linear(x, packed, scales.view(-1).view(torch.uint8)[: 16 * 4], torch.ones((), device=DEV), block=64)
+    assert not ops.nvfp4_linear_supported(x[:, :16], 16, 16) and not ops.int4_linear_supported(x, 256, 16)
+    assert ops.nvfp4_linear_supported(x, 256, 32) and ops.int4_linear_supported(x, 256, 256)
