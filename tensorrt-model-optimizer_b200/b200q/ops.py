@@ -905,13 +905,42 @@ class KvStep(NamedTuple):
     status: torch.Tensor
 
 
-def _int32_vector(t: torch.Tensor, what: str, device=None) -> torch.Tensor:
-    _cuda(t, what)
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+# The wrappers below run once or several times a layer of every decoding step, on kernels of a few microseconds:
+# they read each property of a tensor once, since every such read costs the host 0.1 to 0.3 us.
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """``call`` on torch's current stream of ``device`` (the last argument of the entry point)."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, stream)
+
+
+def _int32_vector(t: torch.Tensor, what: str, device=None) -> int:
+    """Check a contiguous one-dimensional int32 tensor; its number of elements."""
+    if not t.is_cuda:
+        _cuda(t, what)
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"b200q: {what} must be a contiguous one-dimensional int32 tensor")
     if device is not None and t.device != device:
         raise ValueError(f"b200q: {what} is on {t.device}, expected {device}")
-    return t
+    return t.numel()
+
+
+def _table_rows(t: torch.Tensor, requests: int, device):
+    """Check a block table [requests, width] int32 with contiguous rows -> (row stride, width)."""
+    if not t.is_cuda:
+        _cuda(t, "block_table")
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.device != device:
+        raise ValueError("b200q: block_table must be a two-dimensional int32 tensor on the requests' device")
+    n, width = t.shape
+    stride, inner = t.stride()
+    if n != requests or (width > 1 and inner != 1):
+        raise ValueError("b200q: block_table must have one contiguous row per request")
+    return (stride if n > 1 else width), width
 
 
 def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
@@ -924,52 +953,47 @@ def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor
     last request get slot -1.  A request that does not fit (free list, table row, rows, a negative length)
     is refused: it keeps its length, its rows get slot -1, and ``status`` is not zero (bits 1, 2, 8, 4).
     The inputs other than the table stay as they are; repeating the call gives the same result."""
-    lens = _int32_vector(lens, "lens")
-    dev, b = lens.device, lens.numel()
-    new_lens = _int32_vector(new_lens, "new_lens", dev)
-    free_pages = _int32_vector(free_pages, "free_pages", dev)
-    taken = _int32_vector(taken, "taken", dev)
-    _cuda(block_table, "block_table")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("b200q: block_table must be a two-dimensional int32 tensor with contiguous rows")
-    if new_lens.numel() != b or block_table.shape[0] != b or taken.numel() != 1:
-        raise ValueError("b200q: lens, new_lens and block_table must have one entry per request, taken exactly one")
+    b = _int32_vector(lens, "lens")
+    dev = lens.device
+    nfree = _int32_vector(free_pages, "free_pages", dev)
+    if _int32_vector(new_lens, "new_lens", dev) != b or _int32_vector(taken, "taken", dev) != 1:
+        raise ValueError("b200q: lens and new_lens must have one entry per request, taken exactly one")
+    stride, width = _table_rows(block_table, b, dev)
     if b == 0 or page_size <= 0 or tokens < 0:
         raise ValueError("b200q: kv_step needs at least one request, a positive page size and tokens >= 0")
-    if b > 1 and block_table.stride(0) < block_table.shape[1]:
+    if stride < width:
         raise ValueError("b200q: the rows of block_table overlap")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
     ints = torch.empty(2 * b + 3 + tokens, dtype=torch.int32, device=dev)
-    cu, lens_out, taken_out, status, positions = ints.split_with_sizes((b + 1, b, 1, 1, tokens))
     at = ints.data_ptr()
-    with _on(dev):
-        call("b200q_kv_step", lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(),
-             taken.data_ptr(), block_table.data_ptr(), block_table.stride(0) if b > 1 else block_table.shape[1],
-             block_table.shape[1], b, page_size, tokens, slots.data_ptr(), at + 4 * (2 * b + 3), at, at + 4 * (b + 1),
-             at + 4 * (2 * b + 1), at + 4 * (2 * b + 2), _stream(lens))
+    _launch("b200q_kv_step", dev, lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), nfree, taken.data_ptr(),
+            block_table.data_ptr(), stride, width, b, page_size, tokens, slots.data_ptr(), at + 8 * b + 12, at, at + 4 * b + 4,
+            at + 8 * b + 4, at + 8 * b + 8)
+    cu, lens_out, taken_out, status, positions = ints.split_with_sizes((b + 1, b, 1, 1, tokens))
     return KvStep(slots, positions, cu, lens_out, taken_out, status)
 
 
-def _kv_pages(cache, what: str, device=None):
-    """(codes, scales) of one side of a cache, checked -> (codes, scales, pages, heads, page size, dim)."""
+def _kv_pages(cache, what: str, device):
+    """(codes, scales) of one side of a cache, checked -> (codes, scales, shape of the codes)."""
     codes, scales = cache
-    _cuda(codes, what), _cuda(scales, what)
-    if codes.dim() != 4 or codes.dtype != torch.uint8 or scales.element_size() != 1:
+    if not (codes.is_cuda and scales.is_cuda):
+        _cuda(codes, what), _cuda(scales, what)
+    shape = codes.shape
+    if len(shape) != 4 or codes.dtype is not torch.uint8 or scales.element_size() != 1:
         raise ValueError(f"b200q: {what} must be (codes uint8 [pages, heads, page, dim/2], scales float8_e4m3fn "
                          "[pages, heads, page, dim/16])")
-    pages, heads, page, half = codes.shape
-    if scales.shape != (pages, heads, page, half // 8) or half % 8:
+    pages, heads, page, half = shape
+    if half % 8 or scales.shape != (pages, heads, page, half // 8):
         raise ValueError(f"b200q: the scales of {what} do not match its codes")
     if not (codes.is_contiguous() and scales.is_contiguous()):
         raise ValueError(f"b200q: {what} must be contiguous")
-    if codes.device != scales.device or (device is not None and codes.device != device):
+    if codes.device != device or scales.device != device:
         raise ValueError(f"b200q: {what} is on another device")
-    return codes, scales, pages, heads, page, 2 * half
+    return codes, scales, shape
 
 
 def _kv_scale2(s: torch.Tensor, device) -> torch.Tensor:
-    if s.dtype == torch.float32 and s.device == device and s.numel() == 1:
+    if s.dtype is torch.float32 and s.numel() == 1 and s.device == device:
         return s
     s = _amax_f32(s, device)
     if s.numel() != 1:
@@ -977,14 +1001,17 @@ def _kv_scale2(s: torch.Tensor, device) -> torch.Tensor:
     return s
 
 
-def _kv_rows(x: torch.Tensor) -> torch.Tensor:
-    """x [tokens, heads, dim] as the append reads it: last dimension contiguous, 32-byte aligned rows (a view of a
-    fused projection's output usually is; anything else is copied)."""
+def _kv_rows(x: torch.Tensor):
+    """x [tokens, heads, dim] as the append reads it -> (tensor, address, token stride, head stride): last dimension
+    contiguous, 32-byte aligned rows (a view of a fused projection's output usually is; anything else is copied)."""
     es = x.element_size()
-    if (x.stride(2) == 1 and x.stride(0) >= 0 and x.stride(1) >= 0
-            and not ((x.data_ptr() | x.stride(0) * es | x.stride(1) * es) & 31)):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    tok, head, inner = x.stride()
+    at = x.data_ptr()
+    if inner != 1 or (at | tok * es | head * es) & 31:
+        x = x.clone(memory_format=torch.contiguous_format)
+        tok, head, _ = x.stride()
+        at = x.data_ptr()
+    return x, at, tok, head
 
 
 def nvfp4_kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor,
@@ -995,31 +1022,33 @@ def nvfp4_kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cac
     ``v_scale2``: fp32 amax / 2688 of the calibrated amax (a block beyond it saturates).  With ``return_values`` the
     values that the cache now stands for come back as (k, v) in the inputs' dtype, padded rows included: what the
     prompt's own attention reads to agree with later steps."""
-    _cuda(k, "k"), _cuda(v, "v"), _cuda(slots, "slots")
-    dev = k.device
-    kc, ks, pages, heads, page, dim = _kv_pages(k_cache, "k_cache", dev)
-    vc, vs, *vshape = _kv_pages(v_cache, "v_cache", dev)
-    if vshape != [pages, heads, page, dim]:
+    if not (k.is_cuda and v.is_cuda and slots.is_cuda):
+        _cuda(k, "k"), _cuda(v, "v"), _cuda(slots, "slots")
+    dev, shape, dtype = k.device, k.shape, k.dtype
+    kc, ks, cshape = _kv_pages(k_cache, "k_cache", dev)
+    vc, vs, vshape = _kv_pages(v_cache, "v_cache", dev)
+    if vshape != cshape:
         raise ValueError("b200q: k_cache and v_cache differ in shape")
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or v.device != dev or k.shape[1:] != (heads, dim):
+    pages, heads, page, half = cshape
+    dim = 2 * half
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape or v.dtype is not dtype or v.device != dev:
         raise ValueError(f"b200q: k and v must be [tokens, {heads}, {dim}] tensors of one dtype and device")
-    if slots.dtype != torch.int64 or slots.shape != k.shape[:1] or not slots.is_contiguous() or slots.device != dev:
+    tokens = shape[0]
+    if (slots.dtype is not torch.int64 or slots.dim() != 1 or slots.numel() != tokens or not slots.is_contiguous()
+            or slots.device != dev):
         raise ValueError("b200q: slots must be a contiguous int64 tensor with one entry per token")
     dt = dtype_code(k)
-    tokens = k.shape[0]
     kv = vv = None
     if return_values:
-        kv, vv = (torch.empty((tokens, heads, dim), dtype=k.dtype, device=dev) for _ in range(2))
+        kv = torch.empty(shape, dtype=dtype, device=dev)
+        vv = torch.empty(shape, dtype=dtype, device=dev)
     if tokens:
-        k, v = _kv_rows(k), _kv_rows(v)
+        k, k_at, ktok, khead = _kv_rows(k)
+        v, v_at, vtok, vhead = _kv_rows(v)
         k2, v2 = _kv_scale2(k_scale2, dev), _kv_scale2(v_scale2, dev)
-        ktok, khead, _ = k.stride()
-        vtok, vhead, _ = v.stride()
-        with _on(dev):
-            call("b200q_nvfp4_kv_append", k.data_ptr(), ktok, khead, v.data_ptr(), vtok, vhead, dt, slots.data_ptr(), tokens,
-                 heads, dim, k2.data_ptr(), v2.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
-                 pages, page, kv.data_ptr() if return_values else None, vv.data_ptr() if return_values else None,
-                 _stream(k))
+        _launch("b200q_nvfp4_kv_append", dev, k_at, ktok, khead, v_at, vtok, vhead, dt, slots.data_ptr(), tokens, heads, dim,
+                k2.data_ptr(), v2.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), pages, page,
+                kv.data_ptr() if return_values else None, vv.data_ptr() if return_values else None)
     return (kv, vv) if return_values else None
 
 
@@ -1034,7 +1063,7 @@ def _kv_attention_workspace(device: int, *sizes: int) -> int:
 def nvfp4_kv_attention_supported(q: torch.Tensor, heads: int, page: int) -> bool:
     """Whether ``nvfp4_kv_attention`` covers q [tokens, query heads, dim] over a cache of ``heads`` kv heads."""
     return (q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and q.shape[2] in _KV_DIMS
-            and heads > 0 and q.shape[1] % heads == 0 and page > 0 and page % 16 == 0)
+            and heads > 0 and q.shape[1] > 0 and q.shape[1] % heads == 0 and page > 0 and page % 16 == 0)
 
 
 def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor, v_scale2: torch.Tensor,
@@ -1049,52 +1078,51 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
     rows cu_q[b] : cu_q[b + 1], its last tokens, each seeing everything up to itself.  Rows that see nothing are
     zero (lse -inf), and so are rows behind the last request unless ``out`` is given, which keeps them.  ``scale``
     defaults to dim ** -0.5.  Lengths are read on the device: a captured call serves later lengths too."""
-    _cuda(q, "q")
-    dev = q.device
-    kc, ks, pages, heads, page, dim = _kv_pages(k_cache, "k_cache", dev)
-    vc, vs, *vshape = _kv_pages(v_cache, "v_cache", dev)
-    if vshape != [pages, heads, page, dim]:
+    if not q.is_cuda:
+        _cuda(q, "q")
+    dev, shape, dtype = q.device, q.shape, q.dtype
+    kc, ks, cshape = _kv_pages(k_cache, "k_cache", dev)
+    vc, vs, vshape = _kv_pages(v_cache, "v_cache", dev)
+    if vshape != cshape:
         raise ValueError("b200q: k_cache and v_cache differ in shape")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"b200q: nvfp4_kv_attention takes float16 or bfloat16 queries, got {q.dtype}")
-    if not nvfp4_kv_attention_supported(q, heads, page) or q.shape[2] != dim or q.shape[1] == 0:
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise TypeError(f"b200q: nvfp4_kv_attention takes float16 or bfloat16 queries, got {dtype}")
+    pages, heads, page, half = cshape
+    dim = 2 * half
+    if (len(shape) != 3 or shape[2] != dim or dim not in _KV_DIMS or heads == 0 or shape[1] == 0 or shape[1] % heads
+            or page == 0 or page % 16):
         raise ValueError(f"b200q: nvfp4_kv_attention covers q [tokens, n * {heads}, {dim}] with dim 64, 128 or 256 and "
-                         f"page sizes that are multiples of 16; got q {tuple(q.shape)}, page {page}")
-    lens = _int32_vector(lens, "lens", dev)
-    _cuda(block_table, "block_table")
-    b, tokens, qheads = lens.numel(), q.shape[0], q.shape[1]
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev
-            or block_table.shape[0] != b or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise ValueError("b200q: block_table must be int32 [requests, width] with contiguous rows")
+                         f"page sizes that are multiples of 16; got q {tuple(shape)}, page {page}")
+    tokens, qheads, _ = shape
+    b = _int32_vector(lens, "lens", dev)
+    stride, width = _table_rows(block_table, b, dev)
     if cu_q is None:
         if tokens != b:
             raise ValueError("b200q: without cu_q there is one query per request")
-    else:
-        cu_q = _int32_vector(cu_q, "cu_q", dev)
-        if cu_q.numel() != b + 1:
-            raise ValueError("b200q: cu_q must have requests + 1 entries")
+    elif _int32_vector(cu_q, "cu_q", dev) != b + 1:
+        raise ValueError("b200q: cu_q must have requests + 1 entries")
     zero_tail = out is None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    elif out.shape != shape or out.dtype is not dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("b200q: out must be a contiguous, 16-byte aligned tensor like q")
     lse = torch.empty((tokens, qheads), dtype=torch.float32, device=dev) if return_lse else None
     if b == 0 or tokens == 0:
         out.zero_() if zero_tail else None
         return (out, lse.fill_(float("-inf"))) if return_lse else out
-    if q.stride(2) != 1 or (q.data_ptr() | 2 * q.stride(0) | 2 * q.stride(1)) & 15:
+    qtok, qhead, inner = q.stride()
+    if inner != 1 or (q.data_ptr() | 2 * qtok | 2 * qhead) & 15:
         q = q.clone(memory_format=torch.contiguous_format)
+        qtok, qhead, _ = q.stride()
     k2, v2 = _kv_scale2(k_scale2, dev), _kv_scale2(v_scale2, dev)
     group = qheads // heads
-    with _on(dev):
-        need = _kv_attention_workspace(dev.index, tokens, b, heads, group, dim)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)   # this call's own: the allocator orders its reuse
-        call("b200q_nvfp4_kv_attention", q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q), kc.data_ptr(), ks.data_ptr(),
-             vc.data_ptr(), vs.data_ptr(), k2.data_ptr(), v2.data_ptr(), block_table.data_ptr(),
-             block_table.stride(0) if b > 1 else block_table.shape[1], block_table.shape[1], lens.data_ptr(),
-             cu_q.data_ptr() if cu_q is not None else None, b, tokens, heads, group, dim, pages, page,
-             dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr() if return_lse else None,
-             int(zero_tail), ws.data_ptr(), need, _stream(q))
+    need = _kv_attention_workspace(dev.index, tokens, b, heads, group, dim)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)       # this call's own: the allocator orders its reuse
+    _launch("b200q_nvfp4_kv_attention", dev, q.data_ptr(), qtok, qhead, _DT[dtype], kc.data_ptr(), ks.data_ptr(),
+            vc.data_ptr(), vs.data_ptr(), k2.data_ptr(), v2.data_ptr(), block_table.data_ptr(), stride, width, lens.data_ptr(),
+            cu_q.data_ptr() if cu_q is not None else None, b, tokens, heads, group, dim, pages, page,
+            dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr() if return_lse else None,
+            int(zero_tail), ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
@@ -1127,39 +1155,43 @@ def _w4_workspace(device: int, rows: int, n: int, k: int, int4_block: int) -> in
 
 def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, covers, int4_block: int,
                scale2, bias):
-    _cuda(x, "x"), _cuda(packed, "packed"), _cuda(scales, "scales")
-    dev = x.device
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"b200q: products with 4-bit weights take float16 or bfloat16 rows, got {x.dtype}")
+    if not (x.is_cuda and packed.is_cuda and scales.is_cuda):
+        _cuda(x, "x"), _cuda(packed, "packed"), _cuda(scales, "scales")
+    dev, dtype, shape = x.device, x.dtype, x.shape
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise TypeError(f"b200q: products with 4-bit weights take float16 or bfloat16 rows, got {dtype}")
     if packed.dim() != 2 or packed.element_size() != 1:
         raise ValueError("b200q: packed must be [n, k/2] bytes")
-    n, k = packed.shape[0], 2 * packed.shape[1]
+    n, k = packed.shape
+    k *= 2
     if n == 0 or not covers(x, k, block):
-        raise ValueError(f"b200q: no 4-bit product for x {tuple(x.shape)}, weight [{n}, {k}], block {block}")
+        raise ValueError(f"b200q: no 4-bit product for x {tuple(shape)}, weight [{n}, {k}], block {block}")
     if scales.numel() != n * (k // block):
         raise ValueError(f"b200q: expected {n * (k // block)} scales, got {scales.numel()}")
     if packed.device != dev or scales.device != dev or (bias is not None and bias.device != dev):
         raise ValueError("b200q: x, weight and bias must be on one device")
+    bias_at = None
     if bias is not None:
         if bias.numel() != n:
             raise ValueError(f"b200q: bias must have {n} elements")
-        bias = bias.detach().to(x.dtype).contiguous()
+        bias = bias.detach().to(dtype).contiguous()
+        bias_at = bias.data_ptr()
     packed, scales = _prep(packed), scales.contiguous()
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    if x2.stride(1) != 1 or (x2.data_ptr() | 2 * x2.stride(0)) & 15:
+    x2 = x if len(shape) == 2 else x.reshape(-1, k)
+    xs, inner = x2.stride()
+    if inner != 1 or (x2.data_ptr() | 2 * xs) & 15:
         x2 = x2.clone(memory_format=torch.contiguous_format)
-    m, xs = x2.shape[0], x2.stride(0)
-    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
-    most, bias_at = _w4_max_rows(k), bias.data_ptr() if bias is not None else None
+        xs = k
+    m = x2.shape[0]
+    out = torch.empty((*shape[:-1], n), dtype=dtype, device=dev)
+    most, x_at, out_at = _w4_max_rows(k), x2.data_ptr(), out.data_ptr()
     extra = (block,) if scale2 is None else (block, scale2.data_ptr())
-    with _on(dev):
-        for r in range(0, m, most):
-            rows = min(most, m - r)
-            need = _w4_workspace(dev.index, rows, n, k, int4_block)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None    # this call's own
-            call(name, x2.data_ptr() + 2 * r * xs, xs, _DT[x.dtype], packed.data_ptr(), scales.data_ptr(), *extra, bias_at,
-                 out.data_ptr() + 2 * r * n, n, rows, n, k, ws.data_ptr() if need else None, need,
-                 qgemm_status(dev).data_ptr(), _stream(x))
+    for r in range(0, m, most):
+        rows = min(most, m - r)
+        need = _w4_workspace(dev.index, rows, n, k, int4_block)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None        # this call's own
+        _launch(name, dev, x_at + 2 * r * xs, xs, _DT[dtype], packed.data_ptr(), scales.data_ptr(), *extra, bias_at,
+                out_at + 2 * r * n, n, rows, n, k, ws.data_ptr() if need else None, need, qgemm_status(dev).data_ptr())
     return out
 
 

@@ -567,6 +567,16 @@ inline int w4_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 // A round takes a warp's steps in it; one that leaves warps idle is shorter, but not below what a warp needs by itself
 // (0.6); a round that joins warps pays for its barriers, and several CTAs for a launch that adds their sums.
 inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, int& wk, int& ks) {
+  // A decoding loop asks for the same few shapes again and again, and the search costs as much as a launch.
+  struct Entry { int rows, slabs, segs, tiles, sms, wk, ks; };
+  static thread_local Entry seen[64];
+  const uint32_t hash = (rows * 2654435761u) ^ (slabs * 2246822519u) ^ (tiles * 3266489917u) ^ (segs * 668265263u);
+  Entry& e = seen[(hash >> 16) & 63];
+  if (e.rows == rows && e.slabs == slabs && e.segs == segs && e.tiles == tiles && e.sms == sms) {
+    wk = e.wk;
+    ks = e.ks;
+    return ks > 0;
+  }
   const int nt = w4_nt(rows), step = nt == 1 ? W4Ring<1>::kSlabs : W4Ring<2>::kSlabs;
   double best = 1e30;
   for (int c = 1; c <= kW4MaxParts && c <= slabs; ++c) {
@@ -581,6 +591,7 @@ inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, int& wk, i
       if (cost < best) { best = cost; wk = w; ks = c; }
     }
   }
+  e = Entry{rows, slabs, segs, tiles, sms, wk, best < 1e30 ? ks : 0};
   return best < 1e30;
 }
 
