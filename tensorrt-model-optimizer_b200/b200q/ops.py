@@ -1040,8 +1040,8 @@ def nvfp4_kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cac
     dt = dtype_code(k)
     kv = vv = None
     if return_values:
-        kv = torch.empty(shape, dtype=dtype, device=dev)
-        vv = torch.empty(shape, dtype=dtype, device=dev)
+        kv = torch.empty_like(k, memory_format=torch.contiguous_format)
+        vv = torch.empty_like(v, memory_format=torch.contiguous_format)
     if tokens:
         k, k_at, ktok, khead = _kv_rows(k)
         v, v_at, vtok, vhead = _kv_rows(v)
@@ -1103,10 +1103,10 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
         raise ValueError("b200q: cu_q must have requests + 1 entries")
     zero_tail = out is None
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("b200q: out must be a contiguous, 16-byte aligned tensor like q")
-    lse = torch.empty((tokens, qheads), dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty(tokens, qheads, dtype=torch.float32, device=dev) if return_lse else None
     if b == 0 or tokens == 0:
         out.zero_() if zero_tail else None
         return (out, lse.fill_(float("-inf"))) if return_lse else out
@@ -1183,7 +1183,7 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
         x2 = x2.clone(memory_format=torch.contiguous_format)
         xs = k
     m = x2.shape[0]
-    out = torch.empty((*shape[:-1], n), dtype=dtype, device=dev)
+    out = torch.empty(*shape[:-1], n, dtype=dtype, device=dev)
     most, x_at, out_at = _w4_max_rows(k), x2.data_ptr(), out.data_ptr()
     extra = (block,) if scale2 is None else (block, scale2.data_ptr())
     for r in range(0, m, most):
