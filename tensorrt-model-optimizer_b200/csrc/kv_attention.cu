@@ -171,7 +171,7 @@ struct AttnShape {
   static constexpr int kRing = kAttnWarps * kStages * kSlot;
   static constexpr int kMerge = kAttnWarps * kRT * D * 4;
   static constexpr int kSmem = kRing + kMerge;
-  static constexpr int kCtas = D * NT >= 256 ? 2 : 4;                  // per SM
+  static constexpr int kCtas = D * NT >= 256 ? 2 : 3;                  // per SM: registers for two halves in flight
 };
 
 // kRagged: requests may have several queries (cu_q), so that rows of a tile may see different tokens.
@@ -727,7 +727,7 @@ inline int row_tiles(int dim, int tokens, int requests, int group) {
   const int64_t rows = static_cast<int64_t>(group) * ((tokens + requests - 1) / requests);
   return dim < 256 && rows > 8 ? 2 : 1;
 }
-inline int ctas_per_sm(int dim, int nt) { return dim * nt >= 256 ? 2 : 4; }
+inline int ctas_per_sm(int dim, int nt) { return dim * nt >= 256 ? 2 : 3; }
 
 }  // namespace b200q
 
