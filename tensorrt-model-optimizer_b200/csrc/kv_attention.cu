@@ -32,6 +32,7 @@ constexpr int kChunk = 16;                          // tokens of a matrix produc
 constexpr int kStep = 2 * kChunk;                   // tokens a warp handles at a time
 constexpr int kTile = kStep * kAttnWarps;           // tokens of a tile
 constexpr int kSegCost = 2;                         // what beginning and ending a segment costs, in tiles
+constexpr float kNone = -3.0e38f;                   // maximum of a row that has seen nothing: below any score, and finite
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
@@ -253,6 +254,7 @@ kv_attention_kernel(const AttnArgs a) {
   const int* p_row = a.table + pc.b * a.table_stride;
   int p_head = pc.h * a.page;
   const int page_tokens = a.heads * a.page;
+  const bool wide = a.page % kStep == 0;            // the 32 tokens of a step lie in one page: one address, no tail
   uint32_t live = 0;                                // bits 2s, 2s + 1: the halves of slot s that hold (or await) tokens
   int p_slot = 0;
   int p_id[2], p_in[2];                             // page ids of the step's halves (negative: nothing to read), tokens into the page
@@ -263,7 +265,7 @@ kv_attention_kernel(const AttnArgs a) {
     a.chunks_per_page.divmod(p_tok / kChunk, col, in);
     p_in[0] = in * kChunk;
     p_id[0] = __ldg(p_row + col);
-    if (p_tok + kChunk < p_limit) {
+    if (!wide && p_tok + kChunk < p_limit) {
       const bool next = in + 1 == a.chunks_per_page.d;                             // the second half begins the next page
       p_in[1] = next ? 0 : p_in[0] + kChunk;
       p_id[1] = __ldg(p_row + col + next);
@@ -272,6 +274,24 @@ kv_attention_kernel(const AttnArgs a) {
   look_up();
   auto produce = [&]() {
     uint32_t ok = 0;
+    if (wide) {
+      if (static_cast<uint32_t>(p_id[0]) < static_cast<uint32_t>(a.pages)) {
+        ok = 3;                                     // tokens behind the limit are in the page too, and masked below
+        const int64_t row = static_cast<int64_t>(p_id[0]) * page_tokens + (p_head + p_in[0]);
+        const uint8_t* ksrc = a.k_codes + row * (D / 2) + lane * 16;
+        const uint8_t* vsrc = a.v_codes + row * (D / 2) + lane * 16;
+        const uint8_t* ssrc = scale_src + row * (D / 16);
+        const uint32_t dst = ring_addr + p_slot * S::kSlot, sdst = scale_addr + p_slot * S::kSlot;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          copy_async16(dst + i * 512, ksrc + i * 512);
+          copy_async16(dst + S::kCodeBytes + i * 512, vsrc + i * 512);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (lane < 2 * kSide) copy_async16(sdst + c * (S::kScaleBytes / 2), ssrc + c * (S::kScaleBytes / 2));
+      }
+    } else {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       if (static_cast<uint32_t>(p_id[c]) < static_cast<uint32_t>(a.pages)) {
@@ -287,6 +307,7 @@ kv_attention_kernel(const AttnArgs a) {
         }
         if (lane < 2 * kSide) copy_async16(scale_addr + p_slot * S::kSlot + c * (S::kScaleBytes / 2), scale_src + row * (D / 16));
       }
+    }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     live = (live & ~(3u << (2 * p_slot))) | ok << (2 * p_slot);
@@ -358,11 +379,10 @@ kv_attention_kernel(const AttnArgs a) {
       }
     }
     float o[NT][D / 16][4];
-    float m[NT][2], ms[NT][2], l[NT][2];            // ms: m, or 0 while nothing has been seen
+    float m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m[n][0] = m[n][1] = -INFINITY;
-      ms[n][0] = ms[n][1] = 0.f;
+      m[n][0] = m[n][1] = kNone;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
@@ -435,22 +455,25 @@ kv_attention_kernel(const AttnArgs a) {
               }
             }
         }
+        // less[c][n][j]: the scaled score less the row's reference maximum
+        float less[2][NT][4];
         bool grow = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[c][n][j] *= qs[n][j & 1];
-            if (hidden) {
+            for (int j = 0; j < 4; ++j) less[c][n][j] = fmaf(s[c][n][j], qs[n][j & 1], -m[n][j & 1]);
+          if (hidden) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                if (hidden >> (8 * n + 4 * c + j) & 1u) s[c][n][j] = -INFINITY;
-            }
+                if (hidden >> (8 * n + 4 * c + j) & 1u) less[c][n][j] = -INFINITY;
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            grow |= fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])) > m[n][j] + 8.f;
+            grow |= fmaxf(fmaxf(less[0][n][j], less[0][n][j + 2]), fmaxf(less[1][n][j], less[1][n][j + 2])) > 8.f;
         }
         // the reference maximum follows only when a score passes it by 2^8 (P stays within fp16): rarely
         if (__any_sync(0xffffffffu, grow)) {
@@ -458,17 +481,25 @@ kv_attention_kernel(const AttnArgs a) {
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float t = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
+              float t = m[n][j];
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                  if (less[c][n][j + r] != -INFINITY) t = fmaxf(t, s[c][n][j + r] * qs[n][j]);
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-              t = fmaxf(t, m[n][j]);
               const float f = m[n][j] == t ? 1.f : exp2_fast(m[n][j] - t);
               m[n][j] = t;
-              ms[n][j] = t == -INFINITY ? 0.f : t;
               l[n][j] *= f;
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) { o[n][i][j] *= f; o[n][i][j + 2] *= f; }
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                  if (less[c][n][j + r] != -INFINITY) less[c][n][j + r] = fmaf(s[c][n][j + r], qs[n][j], -t);
             }
           }
         }
@@ -477,8 +508,8 @@ kv_attention_kernel(const AttnArgs a) {
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float p0 = exp2_fast(s[c][n][0] - ms[n][0]), p1 = exp2_fast(s[c][n][1] - ms[n][1]);
-            const float p2 = exp2_fast(s[c][n][2] - ms[n][0]), p3 = exp2_fast(s[c][n][3] - ms[n][1]);
+            const float p0 = exp2_fast(less[c][n][0]), p1 = exp2_fast(less[c][n][1]);
+            const float p2 = exp2_fast(less[c][n][2]), p3 = exp2_fast(less[c][n][3]);
             l[n][0] += p0 + p2;
             l[n][1] += p1 + p3;
             pb[c][n][0] = transpose8x8(pack_f16(p0, p1));
@@ -610,7 +641,7 @@ kv_attention_kernel(const AttnArgs a) {
     for (int i = threadIdx.x; i < RT * D / 4; i += kAttnThreads) {
       const int row = i / (D / 4), d = 4 * (i % (D / 4));
       if (row >= rows) continue;
-      float mm = -INFINITY, ll = 0.f;
+      float mm = kNone, ll = 0.f;
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) mm = fmaxf(mm, merge_ml[w][row].x);
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -618,7 +649,7 @@ kv_attention_kernel(const AttnArgs a) {
       for (int w = 0; w < kAttnWarps; ++w) {
         const float2 ml = merge_ml[w][row];
         // a warp that saw nothing weighs nothing; NaN sums stay NaN
-        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : exp2_fast(ml.x - mm);
+        const float f = ml.x == kNone ? (ml.y == 0.f ? 0.f : ml.y) : exp2_fast(ml.x - mm);
         ll += ml.y * f;
         const float4 v = *reinterpret_cast<const float4*>(merge + (w * RT + row) * D + d);
         if (f != 0.f) { acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f; }
@@ -680,12 +711,12 @@ kv_merge_kernel(const AttnArgs a) {
   const int row = blockIdx.y, rr = seg.z * RT + row;
   if (rr >= r.nq * a.group) return;
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  float mm = -INFINITY, ll = 0.f;
+  float mm = kNone, ll = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto join = [&](float2 ml, float4 v) {
     const float t = fmaxf(mm, ml.x);
     const float f0 = mm == t ? 1.f : exp2_fast(mm - t);
-    const float f1 = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : exp2_fast(ml.x - t);
+    const float f1 = ml.x == kNone ? (ml.y == 0.f ? 0.f : ml.y) : exp2_fast(ml.x - t);
     mm = t;
     ll = ll * f0 + ml.y * f1;
     if (f1 == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
