@@ -525,10 +525,12 @@ int b200q_nvfp4_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_
  * q: [tokens, heads * group, dim] of type T (B200Q_F16 or B200Q_BF16) with the given strides (elements,
  * multiples of 8; last dimension contiguous); out contiguous of type T; lse [tokens, heads * group] fp32 (natural
  * logarithm) or NULL.  dim 64, 128 or 256; page a multiple of 16; table rows as in b200q_kv_step (an id outside
- * [0, pages) hides its tokens; lens beyond width * page are cut).  Rows of q at and behind cu_q[requests] are not
- * computed: their output is left as it is, or zeroed (lse -inf) where zero_tail != 0.
+ * [0, pages) hides its tokens; lens beyond width * page are cut).  cu_q is non-decreasing; rows of q in front of
+ * cu_q[0] and from cu_q[requests] on are not computed: their output is left as it is, or zeroed (lse -inf) where
+ * zero_tail != 0.  out must not overlap q.
  * workspace: b200q_nvfp4_kv_attention_workspace(...) bytes, this call's alone until it has run.  Lengths are read on the
- * device only: the call can be captured and replayed with others.  width * page at most 2^30. */
+ * device only: the call can be captured and replayed with others.  width * page and
+ * heads * page at most 2^30. */
 int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
                              const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
                              const uint8_t* v_scales, const float* k_scale2, const float* v_scale2, const int* table,

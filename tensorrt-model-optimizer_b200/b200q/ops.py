@@ -959,8 +959,8 @@ def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor
     if _int32_vector(new_lens, "new_lens", dev) != b or _int32_vector(taken, "taken", dev) != 1:
         raise ValueError("b200q: lens and new_lens must have one entry per request, taken exactly one")
     stride, width = _table_rows(block_table, b, dev)
-    if b == 0 or page_size <= 0 or tokens < 0:
-        raise ValueError("b200q: kv_step needs at least one request, a positive page size and tokens >= 0")
+    if b == 0 or not 0 < page_size <= 1 << 30 or not 0 <= tokens <= 1 << 30:
+        raise ValueError("b200q: kv_step needs at least one request, a positive page size and tokens >= 0 (both up to 2^30)")
     if stride < width:
         raise ValueError("b200q: the rows of block_table overlap")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
@@ -1074,8 +1074,8 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
 
     ``q`` [tokens, query heads, dim] float16 / bfloat16, dim 64, 128 or 256, query heads a multiple of the cache's;
     ``lens`` int32 [requests]: tokens of each request in the cache, the step's own included; ``block_table`` int32
-    [requests, width].  Without ``cu_q`` every request has one query; with it (int32 [requests + 1]) request b owns
-    rows cu_q[b] : cu_q[b + 1], its last tokens, each seeing everything up to itself.  Rows that see nothing are
+    [requests, width].  Without ``cu_q`` every request has one query; with it (int32 [requests + 1], not decreasing)
+    request b owns rows cu_q[b] : cu_q[b + 1], its last tokens, each seeing everything up to itself.  Rows that see nothing are
     zero (lse -inf), and so are rows behind the last request unless ``out`` is given, which keeps them.  ``scale``
     defaults to dim ** -0.5.  Lengths are read on the device: a captured call serves later lengths too."""
     if not q.is_cuda:
@@ -1106,6 +1106,8 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("b200q: out must be a contiguous, 16-byte aligned tensor like q")
+    elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+        raise ValueError("b200q: out must not share q's memory")
     lse = torch.empty(tokens, qheads, dtype=torch.float32, device=dev) if return_lse else None
     if b == 0 or tokens == 0:
         out.zero_() if zero_tail else None

@@ -92,8 +92,8 @@ __device__ __forceinline__ void next_segment(const AttnArgs& a, Cursor& c) {
   if (++c.h < a.heads) return;
   c.h = 0;
   do {
-    if (++c.b >= a.requests) return;
-    c.r = load_request<RT>(a, c.b);
+    if (c.b + 1 >= a.requests) return;              // not reached while the lengths stay what they were at the start
+    c.r = load_request<RT>(a, ++c.b);
   } while (c.r.nrt == 0);
 }
 
@@ -225,7 +225,7 @@ kv_attention_kernel(const AttnArgs a) {
     for (c.b = r0;; ++c.b) {
       c.r = load_request<RT>(a, c.b);
       const int64_t w = request_work(a, c.r);
-      if (t0 < at + w) break;
+      if (t0 < at + w || c.b + 1 >= r1) break;
       at += w;
     }
     const int64_t in = t0 - at;
@@ -233,8 +233,9 @@ kv_attention_kernel(const AttnArgs a) {
     const int64_t seg = in / units;
     start_unit = static_cast<int>(in % units);
     c.kt = max(start_unit - kSegCost, 0);
-    c.rt = static_cast<int>(seg % c.r.nrt);
-    c.h = static_cast<int>(seg / c.r.nrt);
+    // (clamped: should somebody change the lengths while this runs, the result is lost, but nothing leaves its bounds)
+    c.rt = static_cast<int>(seg % max(c.r.nrt, 1));
+    c.h = static_cast<int>(min(seg / max(c.r.nrt, 1), static_cast<int64_t>(a.heads - 1)));
     cc = c;
 #pragma unroll
     for (int w = 0; w < kAttnWarps; ++w) pcs[w] = c;
@@ -696,11 +697,13 @@ kv_merge_kernel(const AttnArgs a) {
   __shared__ float4 acc_s[kGroups][kLanes];
   __shared__ float2 ml_s[kGroups];
   pdl_prologue();
-  if (a.zero_tail) {                                // rows behind the last request of an output allocated by the caller
-    const int64_t from = static_cast<int64_t>(min(max(a.cu_q[a.requests], 0), a.tokens)) * a.heads * a.group;
-    const int64_t to = static_cast<int64_t>(a.tokens) * a.heads * a.group;
-    const int64_t nb = static_cast<int64_t>(gridDim.x) * gridDim.y;
-    for (int64_t r = from + blockIdx.y * gridDim.x + blockIdx.x; r < to; r += nb) {
+  if (a.zero_tail) {                                // rows in front of the first request and behind the last one
+    const int heads = a.heads * a.group;
+    const int64_t head = static_cast<int64_t>(min(max(a.cu_q[0], 0), a.tokens)) * heads;
+    const int64_t tail = static_cast<int64_t>(min(max(a.cu_q[a.requests], 0), a.tokens)) * heads;
+    const int64_t end = head + static_cast<int64_t>(a.tokens) * heads - tail, nb = static_cast<int64_t>(gridDim.x) * gridDim.y;
+    for (int64_t i = blockIdx.y * gridDim.x + blockIdx.x; i < end; i += nb) {
+      const int64_t r = i < head ? i : tail + i - head;
       for (int d = threadIdx.x; d < D; d += 128) static_cast<T*>(a.out)[r * D + d] = Elem<T>::from_float(0.f);
       if (a.lse && threadIdx.x == 0) a.lse[r] = -INFINITY;
     }
@@ -788,7 +791,7 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
   if (!cu_q && tokens != requests) return B200Q_ERR_SHAPE;
   if (dim != 64 && dim != 128 && dim != 256) return B200Q_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(tokens) * group > kFastDivLimit / 2 || static_cast<int64_t>(heads) * group > kFastDivLimit ||
-      static_cast<int64_t>(width) * page > (1 << 30))
+      static_cast<int64_t>(width) * page > (1 << 30) || static_cast<int64_t>(heads) * page > (1 << 30))
     return B200Q_ERR_UNSUPPORTED;
   const uintptr_t align = reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(2 * q_token_stride) |
                           static_cast<uintptr_t>(2 * q_head_stride) | reinterpret_cast<uintptr_t>(k_codes) |

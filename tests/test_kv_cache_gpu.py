@@ -392,6 +392,9 @@ def test_attention_rows_behind_the_last_request():
     want = ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, ln, cu_q=cu)
     out, lse = ops.nvfp4_kv_attention(qp, kc, vc, k2, v2, table, ln, cu_q=cu, return_lse=True)
     assert torch.equal(out[:5], want) and (out[5:] == 0).all() and (lse[5:] == -math.inf).all()
+    # rows in front of the first request as well
+    front, flse = ops.nvfp4_kv_attention(torch.cat([qp[5:], q]), kc, vc, k2, v2, table, ln, cu_q=cu + 4, return_lse=True)
+    assert torch.equal(front[4:], want) and (front[:4] == 0).all() and (flse[:4] == -math.inf).all()
     buf = torch.full_like(qp, 7)
     assert ops.nvfp4_kv_attention(qp, kc, vc, k2, v2, table, ln, cu_q=cu, out=buf) is buf
     assert torch.equal(buf[:5], want) and (buf[5:] == 7).all()
@@ -559,7 +562,7 @@ def test_operators_refuse_what_they_do_not_cover():
     q, kc, vc, k2, v2, table, ln, cu = _attention_case([40, 21], [3, 2], 1, 4, 64, 16, torch.bfloat16)
     with pytest.raises(TypeError):
         ops.nvfp4_kv_attention(q.float(), kc, vc, k2, v2, table, ln, cu_q=cu)
-    for bad in (dict(cu_q=None), dict(cu_q=cu[:-1]), dict(cu_q=cu.long()), dict(cu_q=cu, out=torch.empty_like(q).half())):
+    for bad in (dict(cu_q=None), dict(cu_q=cu[:-1]), dict(cu_q=cu.long()), dict(cu_q=cu, out=torch.empty_like(q).half()), dict(cu_q=cu, out=q)):
         with pytest.raises(ValueError):
             ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, ln, **bad)
     for args in ((q[:, :3, :32], kc, vc, k2, v2, table, ln), (q, (kc[0], kc[1][:, :, :8]), vc, k2, v2, table, ln),
@@ -583,8 +586,9 @@ def test_operators_refuse_what_they_do_not_cover():
                  (one.long(), one, one, one, table[:1]), (ln, ln, one, one, table[:1].expand(2, -1))):
         with pytest.raises(ValueError):
             ops.kv_step(*args, 16, 1)
-    with pytest.raises(ValueError):
-        ops.kv_step(one, one, one, one, table[:1], 0, 1)
+    for page, tokens in ((0, 1), (16, -1), (2 ** 32 + 16, 1), (16, 2 ** 32 + 1)):
+        with pytest.raises(ValueError):
+            ops.kv_step(one, one, one, one, table[:1], page, tokens)
     many = torch.zeros(8193, dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError):
         ops.kv_step(many, many, one, one, torch.zeros(8193, 1, dtype=torch.int32, device=DEV), 16, 1)

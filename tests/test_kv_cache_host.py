@@ -68,7 +68,8 @@ def test_status_codes():
     assert attention(dtype=0) == DTYPE
     for kw in (dict(requests=0), dict(tokens=2), dict(heads=0), dict(group=0), dict(pages=0), dict(page=24), dict(stride=-1), dict(width=-1)):
         assert attention(**kw) == SHAPE, kw
-    assert attention(dim=96) == UNSUPPORTED
+    for kw in (dict(dim=96), dict(width=1 << 20, stride=1 << 20, page=1 << 12), dict(heads=1 << 20, page=1 << 12)):
+        assert attention(**kw) == UNSUPPORTED, kw
     for kw in (dict(q=p + 8), dict(qs=65), dict(qh=4), dict(kc=p + 8), dict(out=p + 4), dict(ws=p + 8)):
         assert attention(**kw) == ALIGN, kw
     assert lib.b200q_nvfp4_kv_attention_workspace(1, 1, 1, 1, 96) == SHAPE
