@@ -565,7 +565,10 @@ inline int w4_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 // How K is cut, over the wk warps of a tile and over ks CTAs: the least of an estimate in steps of a fully loaded SM.
 // A round takes a warp's steps in it; one that leaves warps idle is shorter, but not below what a warp needs by itself
-// (0.6); a round that joins warps pays for its barriers, and several CTAs for a launch that adds their sums.
+// (0.6); a round that joins warps pays for its barriers, several CTAs for a launch that adds their sums, and with more
+// than 8 rows a CTA for putting its part of x into shared memory.  Measured with other choices forced: 16 x 4096 x 4096
+// NVFP4 9.3 us in parts against 11.2 whole, 16 x 8192 x 28672 INT4 41.7 us in 14 parts against 43.6 in 8, 8 x 8192 x 8192
+// INT4 13.2 in 2 parts against 14.9 in more, 1 x 28672 x 8192 NVFP4 31.0 with wk = 1 against 32.2 (4) and 35.7 (16).
 inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, int& wk, int& ks) {
   // A decoding loop asks for the same few shapes again and again, and the search costs as much as a launch.
   struct Entry { int rows, slabs, segs, tiles, sms, wk, ks; };
@@ -578,6 +581,7 @@ inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, int& wk, i
     return ks > 0;
   }
   const int nt = w4_nt(rows), step = nt == 1 ? W4Ring<1>::kSlabs : W4Ring<2>::kSlabs;
+  const double join = nt == 2 ? 1.6 : nt == 4 ? 1.0 : 2.0, fill = nt == 2 ? 0.4 : nt == 4 ? 0.25 : 0.0;
   double best = 1e30;
   for (int c = 1; c <= kW4MaxParts && c <= slabs; ++c) {
     const int part = ((slabs + c - 1) / c + step - 1) / step * step, steps = part / step;
@@ -587,7 +591,8 @@ inline bool w4_cut(int rows, int slabs, int segs, int tiles, int sms, int& wk, i
       const double load = static_cast<double>(tiles) * w / (static_cast<double>(sms / c) * kW4Warps);
       const double whole = floor(load), rest = load - whole;
       const double mine = (steps + w - 1) / w;
-      const double cost = mine * (whole + (rest > 0 ? (rest > 0.6 ? rest : 0.6) : 0)) + ceil(load) * (w > 1 ? 0.15 : 0) + (c > 1 ? 2 : 0);
+      const double cost = mine * (whole + (rest > 0 ? (rest > 0.6 ? rest : 0.6) : 0)) + ceil(load) * (w > 1 ? 0.15 : 0) +
+                          (c > 1 ? join : 0) + fill * ((rows * part / 2 + kW4Warps - 1) / kW4Warps);
       if (cost < best) { best = cost; wk = w; ks = c; }
     }
   }
