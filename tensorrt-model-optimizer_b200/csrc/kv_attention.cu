@@ -48,7 +48,7 @@ struct AttnArgs {
   float* lse;                                       // [tokens, heads * group] or NULL
   float* part;                                      // [ctas, 2, rows, D]
   float2* part_ml;                                  // [ctas, 2, rows]
-  int4* desc;                                       // [ctas]: request, head, row tile, pieces
+  int4* desc;                                       // [ctas][2]: pieces, first query, kv head, first row; rows
   FastDiv chunks_per_page, group_div;
   int width, requests, tokens, heads, group, page, pages, zero_tail;
   float scale;
@@ -187,7 +187,7 @@ kv_attention_kernel(const AttnArgs a) {
   constexpr int VB = D >= 128 ? D / 128 : 1;        // block scales of them
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t scan_sums[kAttnWarps];
-  __shared__ Cursor cc, pcs[kAttnWarps];            // where the CTA's products and each warp's copies are: read between segments only
+  __shared__ Cursor at_segment[2], pcs[kAttnWarps]; // this and the next segment, each warp's copies: read between segments only
   __shared__ int start_unit;                        // of the first segment
   __shared__ float2 merge_ml[kAttnWarps][RT];
 
@@ -215,7 +215,7 @@ kv_attention_kernel(const AttnArgs a) {
   }
   const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total / (kSegCost + 1)), cta = blockIdx.x;
   if (cta >= ctas) {
-    if (threadIdx.x == 0) a.desc[cta] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) a.desc[2 * cta] = make_int4(0, 0, 0, 0);
     return;
   }
   const int64_t t0 = cta * total / ctas, t1 = (cta + 1) * total / ctas;
@@ -236,7 +236,7 @@ kv_attention_kernel(const AttnArgs a) {
     // (clamped: should somebody change the lengths while this runs, the result is lost, but nothing leaves its bounds)
     c.rt = static_cast<int>(seg % max(c.r.nrt, 1));
     c.h = static_cast<int>(min(seg / max(c.r.nrt, 1), static_cast<int64_t>(a.heads - 1)));
-    cc = c;
+    at_segment[0] = c;
 #pragma unroll
     for (int w = 0; w < kAttnWarps; ++w) pcs[w] = c;
   }
@@ -332,32 +332,42 @@ kv_attention_kernel(const AttnArgs a) {
   int left = p_left0;
   int slot = 0;
   int4 my_desc = make_int4(0, 0, 0, 0);
+  int my_rows = 0;
 
-  while (left > 0) {
-    // ---- one segment, or this CTA's part of it ----
-    const int kt_end = min(cc.r.nkt, cc.kt + left);
-    const int row0 = cc.rt * RT, rows = min(cc.r.nq * a.group - row0, RT);
-    const int lim_lo = row_limit(a, cc.r, row0), lim_hi = row_limit(a, cc.r, row0 + rows - 1);
-    // queries: thread (gr, qd) holds dimensions qd * D/4 ... of row gr of each 8-row tile, as fp16 times 2^k
-    uint32_t qf[NT][D / 8];
-    float qs[NT][2];
+  // queries: thread (gr, qd) holds dimensions qd * D/4 ... of row gr of each 8-row tile
+  uint32_t qf[NT][D / 8];
+  auto load_q = [&](const Cursor& c) {
+    const int first = c.rt * RT, rows = min(c.r.nq * a.group - first, RT);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 8 * n + gr;
-      float back = 1.f;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) qf[n][i] = 0;
       if (8 * n + gr < rows) {
         uint32_t tok, hd;
-        a.group_div.divmod(row, tok, hd);
-        hd += cc.h * a.group;
-        const T* src = static_cast<const T*>(a.q) + (cc.r.q0 + tok) * a.q_token_stride + hd * a.q_head_stride + qd * (D / 4);
+        a.group_div.divmod(first + 8 * n + gr, tok, hd);
+        hd += c.h * a.group;
+        const T* src = static_cast<const T*>(a.q) + (c.r.q0 + tok) * a.q_token_stride + hd * a.q_head_stride + qd * (D / 4);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-          const uint4 v = reinterpret_cast<const uint4*>(src)[i];
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
           qf[n][4 * i] = v.x; qf[n][4 * i + 1] = v.y; qf[n][4 * i + 2] = v.z; qf[n][4 * i + 3] = v.w;
         }
       }
+    }
+  };
+  load_q(at_segment[0]);
+
+#pragma unroll 1
+  for (int which = 0; left > 0; which ^= 1) {
+    // ---- one segment, or this CTA's part of it ----
+    const Cursor& cc = at_segment[which];
+    const int kt_end = min(cc.r.nkt, cc.kt + left);
+    const int row0 = cc.rt * RT, rows = min(cc.r.nq * a.group - row0, RT);
+    const int lim_lo = row_limit(a, cc.r, row0), lim_hi = row_limit(a, cc.r, row0 + rows - 1);
+    float qs[NT][2];                                // q becomes fp16 times 2^k of its row
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float back = 1.f;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         uint32_t top = 0;                           // largest finite |q| of the row, as a bf16 pattern
 #pragma unroll
@@ -635,8 +645,15 @@ kv_attention_kernel(const AttnArgs a) {
         for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[n][i][j], o[n][i][j + 2]);
       }
     }
-    __syncthreads();
     const bool first_piece = cc.kt == 0, last_piece = kt_end == cc.r.nkt;
+    left -= kt_end - cc.kt + kSegCost;
+    if (threadIdx.x == 0 && left > 0) {
+      Cursor next = cc;
+      next_segment<RT>(a, next);
+      at_segment[which ^ 1] = next;
+    }
+    __syncthreads();
+    if (left > 0) load_q(at_segment[which ^ 1]);    // on its way while the warps' parts are joined
     const bool whole = first_piece && last_piece;
     const int piece = first_piece ? 1 : 0;          // slot 0: the segment began in an earlier CTA
     for (int i = threadIdx.x; i < RT * D / 4; i += kAttnThreads) {
@@ -674,28 +691,29 @@ kv_attention_kernel(const AttnArgs a) {
     if (first_piece && !last_piece) {               // the pieces that follow belong to the next CTAs, one each
       const int64_t seg_last = t1 + (cc.r.nkt - kt_end) - 1;
       const int64_t owner = ((seg_last + 1) * ctas - 1) / total;
-      my_desc = make_int4(cc.b, cc.h, cc.rt, static_cast<int>(owner - cta + 1));
+      my_desc = make_int4(static_cast<int>(owner - cta + 1), cc.r.q0, cc.h, row0);
+      my_rows = rows;
     }
-    left -= kt_end - cc.kt + kSegCost;
-    __syncthreads();
-    if (left > 0) {
-      if (threadIdx.x == 0) next_segment<RT>(a, cc);
-      __syncthreads();
-    }
+    __syncthreads();                                // read before the next segment's parts are written
   }
-  if (threadIdx.x == 0) a.desc[cta] = my_desc;
+  if (threadIdx.x == 0) {
+    a.desc[2 * cta] = my_desc;
+    a.desc[2 * cta + 1] = make_int4(my_rows, 0, 0, 0);
+  }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Pieces of the segments that span several CTAs, joined in the order of the CTAs.  Block (c, row): the segment
-// that begins in CTA c's share and ends in a later one.  The threads split into groups of D/4 that take every
-// fourth piece (or so) and meet in shared memory.
+// that begins in CTA c's share and ends in a later one.  All pieces' maxima and sums first, which gives every piece
+// its weight; then groups of D/4 threads add up every kGroups-th piece, with loads that depend on nothing.
+constexpr int kMergeMost = 2048;                    // CTAs, hence pieces, at most
+
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(128)
 kv_merge_kernel(const AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 128 / kLanes;
   __shared__ float4 acc_s[kGroups][kLanes];
-  __shared__ float2 ml_s[kGroups];
+  __shared__ float weight[kMergeMost], red[2][4];
   pdl_prologue();
   if (a.zero_tail) {                                // rows in front of the first request and behind the last one
     const int heads = a.heads * a.group;
@@ -708,35 +726,49 @@ kv_merge_kernel(const AttnArgs a) {
       if (a.lse && threadIdx.x == 0) a.lse[r] = -INFINITY;
     }
   }
-  const int4 seg = a.desc[blockIdx.x];
-  if (seg.w == 0) return;
-  const Request r = load_request<RT>(a, seg.x);
-  const int row = blockIdx.y, rr = seg.z * RT + row;
-  if (rr >= r.nq * a.group) return;
+  const int4 seg = a.desc[2 * blockIdx.x];
+  const int row = blockIdx.y, pieces = seg.x;
+  if (pieces == 0 || row >= a.desc[2 * blockIdx.x + 1].x) return;
+  auto slot_of = [&](int i) { return (static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * RT + row; };
+  const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
+  float mm = kNone;
+  for (int i = threadIdx.x; i < pieces; i += 128) mm = fmaxf(mm, a.part_ml[slot_of(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  if (lane32 == 0) red[0][warp] = mm;
+  __syncthreads();
+  mm = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float ll = 0.f;
+  for (int i = threadIdx.x; i < pieces; i += 128) {
+    const float2 ml = a.part_ml[slot_of(i)];
+    // a piece that saw nothing weighs nothing; NaN sums stay NaN
+    const float f = ml.x == kNone ? (ml.y == 0.f ? 0.f : ml.y) : exp2_fast(ml.x - mm);
+    weight[i] = f;
+    ll += ml.y * f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+  if (lane32 == 0) red[1][warp] = ll;
+  __syncthreads();
+  ll = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  float mm = kNone, ll = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto join = [&](float2 ml, float4 v) {
-    const float t = fmaxf(mm, ml.x);
-    const float f0 = mm == t ? 1.f : exp2_fast(mm - t);
-    const float f1 = ml.x == kNone ? (ml.y == 0.f ? 0.f : ml.y) : exp2_fast(ml.x - t);
-    mm = t;
-    ll = ll * f0 + ml.y * f1;
-    if (f1 == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-    acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1;
-    acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
-  };
-#pragma unroll 4
-  for (int i = grp; i < seg.w; i += kGroups) {
-    const int64_t p = (static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * RT + row;
-    join(a.part_ml[p], *reinterpret_cast<const float4*>(a.part + p * D + 4 * lane));
+#pragma unroll 8
+  for (int i = grp; i < pieces; i += kGroups) {
+    const float f = weight[i];
+    const float4 v = *reinterpret_cast<const float4*>(a.part + slot_of(i) * D + 4 * lane);
+    if (f != 0.f) { acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f; }
   }
   acc_s[grp][lane] = acc;
-  if (lane == 0) ml_s[grp] = make_float2(mm, ll);
   __syncthreads();
   if (grp) return;
-  for (int g = 1; g < kGroups; ++g) join(ml_s[g], acc_s[g][lane]);
-  const int64_t at = static_cast<int64_t>(r.q0 + rr / a.group) * (a.heads * a.group) + seg.y * a.group + rr % a.group;
+  for (int g = 1; g < kGroups; ++g) {
+    const float4 v = acc_s[g][lane];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  uint32_t tok, hd;
+  a.group_div.divmod(seg.w + row, tok, hd);
+  const int64_t at = static_cast<int64_t>(seg.y + tok) * (a.heads * a.group) + seg.z * a.group + hd;
   const float f = ll == 0.f ? 0.f : __fdividef(__ldg(a.v_scale2), ll);
   uint2 packed;
   packed.x = Elem<T>::pack2(acc.x * f, acc.y * f);
@@ -771,7 +803,7 @@ extern "C" int64_t b200q_nvfp4_kv_attention_workspace(int tokens, int requests, 
   if (tokens <= 0 || requests <= 0 || heads <= 0 || group <= 0 || (dim != 64 && dim != 128 && dim != 256)) return B200Q_ERR_SHAPE;
   const int nt = row_tiles(dim, tokens, requests, group);
   const int64_t ctas = static_cast<int64_t>(sm_count_cached()) * ctas_per_sm(dim, nt);
-  return ctas * (16 + 2 * 8 * nt * (4 * static_cast<int64_t>(dim) + 8));
+  return ctas * (32 + 2 * 8 * nt * (4 * static_cast<int64_t>(dim) + 8));
 }
 
 extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
@@ -801,7 +833,7 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
   if (align & 15u) return B200Q_ERR_ALIGN;
   if (workspace_bytes < b200q_nvfp4_kv_attention_workspace(tokens, requests, heads, group, dim)) return B200Q_ERR_CAPACITY;
   const int nt = row_tiles(dim, tokens, requests, group);
-  const int ctas = sm_count_cached() * ctas_per_sm(dim, nt);
+  const int ctas = min(sm_count_cached() * ctas_per_sm(dim, nt), kMergeMost);
   AttnArgs a{};
   a.q = q; a.q_token_stride = q_token_stride; a.q_head_stride = q_head_stride;
   a.k_codes = k_codes; a.k_scales = k_scales; a.v_codes = v_codes; a.v_scales = v_scales;
@@ -809,7 +841,7 @@ extern "C" int b200q_nvfp4_kv_attention(const void* q, int64_t q_token_stride, i
   a.table = table; a.table_stride = table_stride; a.lens = lens; a.cu_q = cu_q;
   a.out = out; a.lse = lse;
   a.desc = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(a.desc + ctas);
+  a.part = reinterpret_cast<float*>(a.desc + 2 * ctas);
   a.part_ml = reinterpret_cast<float2*>(a.part + static_cast<int64_t>(ctas) * 2 * 8 * nt * dim);
   a.width = width; a.requests = requests; a.tokens = tokens; a.heads = heads; a.group = group;
   a.page = page; a.pages = pages; a.zero_tail = cu_q ? zero_tail : 0;
