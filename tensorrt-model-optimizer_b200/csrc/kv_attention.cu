@@ -6,8 +6,9 @@
 // Work.  A segment is one kv head of one request and one tile of 8 NT query rows (query tokens x the heads
 // that share the kv head); its cache tokens are cut into tiles of 128.  All tiles of all segments, each segment
 // preceded by kSegCost units for beginning and ending it, form one line that is dealt out to the CTAs in equal
-// contiguous shares, so ragged lengths balance without the host knowing a length.  A segment that lies inside one share is finished there; pieces of the others go to a workspace as
-// (max, sum, unnormalised output) and kv_merge_kernel joins them in a fixed order.
+// contiguous shares, so ragged lengths balance without the host knowing a length.  A segment that lies inside one
+// share is finished there; pieces of the others go to a workspace as (max, sum, unnormalised output) and
+// kv_merge_kernel joins them in a fixed order.
 //
 // Inside a CTA the four warps take 32 tokens of each tile.  A warp fetches its codes and scales (2 KB + 256 B each for
 // K and V at D = 128) with cp.async into a ring of its own, two steps deep, with the page ids read ahead; there is no
@@ -17,11 +18,12 @@
 // rows, the query rows the 8 columns, so a group of up to eight heads wastes nothing.  E2M1 times E4M3 has at
 // most six significant bits and lies in [2^-10, 2688]: K and V without the per-tensor scale are EXACT in fp16.
 // q is multiplied by a power of two per row that brings its largest element to [2^14, 2^15): bf16 elements stay
-// exact in fp16 down to 2^-29 of the row's largest.  The only rounding besides fp32 accumulation is P to fp16
-// (2^-11 relative); the softmax sum takes the unrounded fp32 values.  The order of the head dimension inside a
-// product and of the tokens inside a tile is free, so a thread's operand is one contiguous run of the row:
-// D/4 dimensions of one token for K, D/8 dimensions of four tokens for V, whose nibbles are interleaved so that
-// one conversion gives the same dimension of two neighbouring tokens.
+// exact in fp16 down to 2^-29 of the row's largest.  The only rounding besides fp32 accumulation is P to fp16:
+// 2^-11 relative, and 2^-36 of the largest weight below fp16's normal range (P is 2^11 at the reference maximum, so
+// that the many small weights of a long request are not lost); the softmax sum takes the unrounded fp32 values.
+// The order of the head dimension inside a product and of the tokens inside a tile is free, so a thread's operand is
+// one contiguous run of the row: D/4 dimensions of one token for K, D/8 dimensions of four tokens for V, whose nibbles
+// are interleaved so that one conversion gives the same dimension of two neighbouring tokens.
 //
 // What bounds it.  The fetches alone run at 6.3 TB/s (0.95 of the copy rate); with the products 4.2 to 4.8 TB/s: 295
 // instructions per 16 tokens of a head of 128, 64 of them conversions and 64 multiplies that issue every other cycle, at
@@ -39,6 +41,7 @@ constexpr int kChunk = 16;                          // tokens of a matrix produc
 constexpr int kStep = 2 * kChunk;                   // tokens a warp handles at a time
 constexpr int kTile = kStep * kAttnWarps;           // tokens of a tile
 constexpr int kSegCost = 2;                         // what beginning and ending a segment costs, in tiles
+constexpr float kBase = 11.f, kTop = 15.f;          // log2 P at the reference maximum, and the most that P may reach
 constexpr float kNone = -3.0e38f;                   // maximum of a row that has seen nothing: below any score, and finite
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -473,7 +476,7 @@ kv_attention_kernel(const AttnArgs a) {
               }
             }
         }
-        // less[c][n][j]: the scaled score less the row's reference maximum
+        // less[c][n][j]: log2 P, the scaled score less the row's reference (kBase below a maximum of its scores)
         float less[2][NT][4];
         bool grow = false;
 #pragma unroll
@@ -491,15 +494,15 @@ kv_attention_kernel(const AttnArgs a) {
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            grow |= fmaxf(fmaxf(less[0][n][j], less[0][n][j + 2]), fmaxf(less[1][n][j], less[1][n][j + 2])) > 8.f;
+            grow |= fmaxf(fmaxf(less[0][n][j], less[0][n][j + 2]), fmaxf(less[1][n][j], less[1][n][j + 2])) > kTop;
         }
-        // the reference maximum follows only when a score passes it by 2^8 (P stays within fp16): rarely
+        // the reference follows only when a score passes the maximum by 2^4 (P stays within fp16): rarely
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float t = m[n][j];
+              float t = kNone;
 #pragma unroll
               for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -508,6 +511,7 @@ kv_attention_kernel(const AttnArgs a) {
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+              t = fmaxf(m[n][j], t - kBase);
               const float f = m[n][j] == t ? 1.f : exp2_fast(m[n][j] - t);
               m[n][j] = t;
               l[n][j] *= f;

@@ -325,6 +325,36 @@ def test_attention_query_magnitudes(q_scale):
     _check_attention([100, 33], [1, 1], 2, 4, 128, 16, torch.bfloat16, scale=0.05 / q_scale, q_scale=q_scale)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_many_small_weights_beside_a_large_one(dim):
+    """One token whose weight is 1 and very many of 2^-26 to 2^-24 each: together they are part of the output.  The
+    values' average shows what is lost: V is 1 for the one, -400 for the others.  Enough requests (of the same pages)
+    that each is handled in one piece."""
+    from b200q import ops
+
+    page, tokens, b = 64, 40000, 1000
+    pages = -(-tokens // page)
+    kc, vc = _cache(pages, 1, page, dim), _cache(pages, 1, page, dim)
+    k, v = torch.zeros(tokens, 1, dim, device=DEV), torch.full((tokens, 1, dim), -400.0, device=DEV)
+    k[0, 0, 0], v[0] = 6, 1
+    k2, v2 = torch.tensor(1 / 448, device=DEV), torch.tensor(1 / 4, device=DEV)
+    ops.nvfp4_kv_append(k, v, torch.arange(tokens, device=DEV), kc, vc, k2, v2)
+    q = torch.zeros(b, 1, dim, dtype=torch.float16, device=DEV)
+    q[:, 0, 0] = 1
+    table, lens = torch.arange(pages, dtype=torch.int32, device=DEV).expand(b, pages), _i32([tokens] * b)
+    z = _dequantised(kc, k2).flatten(0, 2)[:tokens, 0]
+    for bits in (24.5, 25.5):
+        scale = bits * math.log(2) / float(z[0])
+        p = torch.softmax(z * scale, 0)
+        ref = p @ _dequantised(vc, v2).flatten(0, 2)[:tokens]
+        out = ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, lens, scale=scale)[:, 0].double()
+        # the output's half step; 2^-11 of each weight, 2^-36 of the largest where that is less; the exponent's rounding (25 * 2^-23 and the scale's 2^-24), the
+        # sums in fp32 (chains of 40000 / 128 steps of a warp, each with two products of 16 tokens: below 1000 additions)
+        size = p @ _dequantised(vc, v2).flatten(0, 2)[:tokens].abs()
+        tol = 2.0 ** -11 * ref.abs() + size * (2.0 ** -11 + 25 * 2.0 ** -22 + 1000 * 2.0 ** -23) + tokens * 400 * 2.0 ** -36
+        assert float(((out - ref).abs() - tol).max()) <= 0
+
+
 def test_attention_scale_may_be_negative():
     _check_attention([70, 9], [1, 2], 1, 4, 64, 16, torch.float16, scale=-0.2)
 
