@@ -56,13 +56,25 @@ def enable_real_quant_gemm(model: nn.Module, weight_only: bool = False) -> None:
     real-quant GEMM.  ``weight_only`` marks those too whose weight quantiser alone is enabled: with a packed
     4-bit weight and few rows they then read the packed weight instead of dequantising it first."""
     for module in model.modules():
-        if _both_quantizers_enabled(module) or (weight_only and _only_weight_quantizer_enabled(module)):
+        if _both_quantizers_enabled(module):
+            _set_weight_only(module, False)
             module._use_real_quant_gemm = True
+        elif weight_only and _only_weight_quantizer_enabled(module):
+            _set_weight_only(module, True)
+            module._use_real_quant_gemm = True
+
+
+def _set_weight_only(module: nn.Module, value: bool) -> None:
+    """A layer whose mark changes asks the registry again: what it remembers was matched for the other mark."""
+    if getattr(module, "_weight_only_gemm", False) != value:
+        module._weight_only_gemm = value
+        module.__dict__.pop("_real_quant_gemm_impl", None)
 
 
 def disable_real_quant_gemm(model: nn.Module) -> None:
     for module in model.modules():
         if hasattr(module, "_use_real_quant_gemm"):
+            _set_weight_only(module, False)
             module._use_real_quant_gemm = False
 
 

@@ -43,6 +43,8 @@ def _covered(module, input) -> bool:
     kind, shape, dtype = (weight.metadata[key] for key in ("qtensor_class", "shape", "dtype"))
     if kind not in (INT4QTensor, NVFP4QTensor) or len(shape) != 2 or dtype != input.dtype or input.shape[-1] != shape[1]:
         return False
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != dtype:   # F.linear would cast both
+        return False
     block = (getattr(wq, "block_sizes", None) or {}).get(-1)
     if not isinstance(block, int) or weight.data.numel() * 2 != shape[0] * shape[1]:      # padded rows
         return False
@@ -57,8 +59,8 @@ def _weight_only_availability_check(module, input, args, kwargs) -> bool:
     if not (isinstance(module, RealQuantLinear) and isinstance(getattr(module, "input_quantizer", None), TensorQuantizer)
             and isinstance(getattr(module, "weight_quantizer", None), TensorQuantizer)):
         return False
-    return (not module.input_quantizer.is_enabled and module.weight_quantizer.is_enabled and torch.cuda.is_available()
-            and input.is_cuda and _covered(module, input))
+    return (getattr(module, "_weight_only_gemm", False) and not module.input_quantizer.is_enabled
+            and module.weight_quantizer.is_enabled and torch.cuda.is_available() and input.is_cuda and _covered(module, input))
 
 
 class WeightOnlyLinear(Function):

@@ -103,6 +103,42 @@ def test_switching_on_and_off():
     assert torch.equal(model(x), plain) and not torch.equal(fast, plain)
 
 
+def test_layers_that_are_not_marked_keep_their_gemm():
+    """An NVFP4 layer whose input quantiser is switched off after compress runs what it ran before."""
+    import b200q as mtq
+    from b200q import ops
+
+    torch.manual_seed(0)
+    layer = nn.Sequential(nn.Linear(256, 64)).bfloat16().cuda()
+    x = torch.randn(4, 256, device=DEV, dtype=torch.bfloat16)
+    mtq.quantize(layer, copy.deepcopy(mtq.NVFP4_DEFAULT_CFG), lambda m: m(x))
+    mtq.compress(layer)
+    want = layer(x)
+    del layer[0]._real_quant_gemm_impl
+    mtq.disable_quantizer(layer, "*input_quantizer")
+    assert torch.equal(layer(x), want)
+    mtq.backends.enable_real_quant_gemm(layer, weight_only=True)
+    got = layer(x)
+    m = layer[0]
+    assert torch.equal(got, ops.nvfp4_linear(x, m.weight.data, m.weight_quantizer._scale, m.weight_quantizer._double_scale, m.bias))
+    mtq.enable_quantizer(layer, "*input_quantizer")
+    mtq.backends.enable_real_quant_gemm(layer)                     # both enabled again: the layer's own GEMM again
+    assert torch.equal(layer(x), want)
+
+
+def test_autocast_to_another_type():
+    import b200q as mtq
+
+    torch.manual_seed(0)
+    layer = nn.Sequential(nn.Linear(256, 64)).half().cuda()
+    mtq.quantize(layer, copy.deepcopy(mtq.INT4_BLOCKWISE_WEIGHT_ONLY_CFG), lambda m: None)
+    mtq.compress(layer, {"weight_only_gemm": True})
+    x = torch.randn(4, 256, device=DEV, dtype=torch.float16)
+    assert layer(x).dtype == torch.float16
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert layer(x).dtype == torch.bfloat16
+
+
 def test_other_types_and_empty_inputs_fall_back():
     import b200q as mtq
 
