@@ -10,9 +10,10 @@
 //
 // Mathematics.  mma.m16n8k16 with 16 weight rows as the rows and 8 rows of x as the columns.  code - 8 is an exact
 // fp16 (1024 + code, minus 1032), and e2m1 * e4m3 is one too (six significant bits, [2^-10, 2688]); the INT4 scale
-// multiplies the fp32 sum of its group, scale2 the result.  x in bf16 is multiplied by a power of two per row that
-// brings the largest element of the CTA's part to [2^14, 2^15): exact in fp16 down to 2^-29 of it, and below that
-// off by less than 2^-39 of it, far under the 2^-24 of the fp32 sums.  The k order inside a product is free, so a
+// multiplies the fp32 sum of its group, scale2 the result.  x in bf16, and in fp16 where half of it is divided by 16
+// (INT4), is multiplied by a power of two per row that brings the largest element of the CTA's part to [2^14, 2^15):
+// exact in fp16 down to 2^-29 of it (2^-25 where divided), and below that off by less than 2^-35 of it, far under the
+// 2^-24 of the fp32 sums.  The k order inside a product is free, so a
 // lane's operand is a contiguous run of the packed row and x is put into shared memory in that order.
 //
 // Work.  A CTA of 16 warps has an SM to itself, with its part of x in shared memory: all of K, or one of ks parts
@@ -151,6 +152,8 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   constexpr int kPart = kW4Rows * 8 * NT;           // partial sums of a warp
   constexpr int kStep = W4Ring<NT>::kSlabs, kStages = W4Ring<NT>::kStages, kStageBytes = W4Ring<NT>::kBytes;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool kScaled = kBf16 || FMT == kFmtInt4;       // x is multiplied by a power of two per row
+  constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint32_t xmax[8 * NT];
   __shared__ int not_finite, xbad[8 * NT];          // INT4: x (a row of it) holds an infinity or a NaN
@@ -287,26 +290,30 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
   auto max_x = [&](int u, const uint4& v) {
     uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
     m = max(m & 0xffffu, m >> 16);
-    if (m >= 0x7f80u) {                             // infinity or NaN: the largest of the others
+    if (m >= kInf) {                                // infinity or NaN: the largest of the others
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       m = 0;
       for (int j = 0; j < 4; ++j) {
         const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
-        m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+        m = max(m, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
       }
     }
     m = warp_max_u32(m);
     if (lane == 0 && m) atomicMax(&xmax[a.pairs.div(u)], m);
+  };
+  // log2 of the power: from the biased exponent, kept where the power and its inverse are normal numbers
+  auto row_shift = [&](uint32_t top) {
+    return kBf16 ? 14 + 127 - max(static_cast<int>(top >> 7), 28) : max(14 + 15 - max(static_cast<int>(top >> 10), 1), 0);
   };
   auto store_x = [&](int u, const uint4& v) {
     uint32_t row, pair;
     a.pairs.divmod(u, row, pair);
     const int slab = 2 * pair + (lane >> 4);
     uint32_t h[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (kBf16) {
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - max(static_cast<int>(xmax[row] >> 7), 28)) << 23);
+    if constexpr (kScaled) {
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + row_shift(xmax[row])) << 23);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
+      for (int j = 0; j < 4; ++j) h[j] = w4_pack_f16(w4_half_word<T>(h[j], 0) * up, w4_half_word<T>(h[j], 1) * up);
     }
     uint4 o;
     if constexpr (FMT == kFmtInt4) {
@@ -334,13 +341,12 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
     *reinterpret_cast<uint4*>(xs + (((slab * a.rows + static_cast<int>(row)) * 4 + (x_i ^ (row & 1))) * 4 + x_q) * 16) = o;
   };
   uint4 hold[kHold];
-  if constexpr (!kBf16 && FMT == kFmtInt4) __syncthreads();   // not_finite is 0
 #pragma unroll
   for (int j = 0; j < kHold; ++j) {
     if (warp + j * kW4Warps >= units) break;
     hold[j] = load_x(warp + j * kW4Warps);
   }
-  if constexpr (kBf16) {
+  if constexpr (kScaled) {
     if (threadIdx.x < 8 * NT) xmax[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
@@ -369,8 +375,8 @@ w4_linear_kernel(const __grid_constant__ CUtensorMap map, const W4Args a) {
     for (int j = 0; j < 2; ++j) {
       const int row = 8 * n + 2 * qd + j;
       back[n][j] = 1.f;
-      if constexpr (kBf16)
-        if (row < a.rows) back[n][j] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(xmax[row] >> 7), 28) - 14) << 23);
+      if constexpr (kScaled)
+        if (row < a.rows) back[n][j] = __uint_as_float(static_cast<uint32_t>(127 - row_shift(xmax[row])) << 23);
     }
 
   auto store = [&](int row, int col, float sum) {

@@ -35,7 +35,8 @@ def _nvfp4(n, k, dtype, seed, block=16):
 def _close(out, x, w, bias=None):
     """Half a step of the output's type, the fp32 sums (k + 8 operations, each off by at most 2^-23 of the sum of
     magnitudes; the tensor core may truncate where it adds), the group's reciprocal and its product (2^-22), and x's
-    smallest elements in fp16 (2^-38 of the row's largest)."""
+    smallest elements in fp16 (2^-38 of the row's largest).  Results beyond the type's largest number are infinite: both
+    sides are compared cut off there."""
     ref = x.double() @ w.t()
     size = x.double().abs() @ w.abs().t()
     if bias is not None:
@@ -45,7 +46,8 @@ def _close(out, x, w, bias=None):
     tol = (info.eps / 2 * ref.abs().clamp(min=info.tiny) + size * ((x.shape[-1] + 8) * 2.0 ** -23 + 2.0 ** -21)
            + 2.0 ** -38 * x.double().abs().amax(-1, keepdim=True) * w.abs().sum(1)) * 1.01
     assert out.shape == ref.shape
-    assert float(((out.double() - ref).abs() - tol).max()) <= 0
+    out, ref = (t.clamp(-info.max, info.max) for t in (out.double(), ref))
+    assert float(((out - ref).abs() - tol).max()) <= 0
 
 
 def _x(m, k, dtype, seed=0):
@@ -135,6 +137,28 @@ def test_bf16_rows_of_any_magnitude(scale):
     _close(ops.nvfp4_linear(x, packed, scales, s2), x, w)
     packed, scales, w = _int4(40, 1024, 128, torch.bfloat16, seed=2)
     _close(ops.int4_linear(x, packed, scales, 128), x, w)
+
+
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 9, 20])
+def test_fp16_rows_of_any_magnitude(m, block):
+    """Rows from the smallest numbers of the type (2^-24 and few bits) to its largest, each as exact as the others.  The
+    weights are large enough for the smallest rows' results to be normal numbers."""
+    from b200q import ops
+
+    g = torch.Generator(device=DEV).manual_seed(m)
+    w = (torch.randn(40, 1024, generator=g, device=DEV) * 100).half()
+    packed, scales = ops.int4_quantize(w.reshape(-1), block)
+    packed = packed.reshape(40, 512)
+    c = torch.stack((packed >> 4, packed & 15), -1).reshape(40, 1024 // block, block).double()
+    w = ((c - 8) / scales.reshape(40, -1, 1).double()).reshape(40, 1024)
+    size = torch.logspace(-24, 0, m, base=2, device=DEV).unsqueeze(1)
+    x = (torch.randn(m, 1024, generator=g, device=DEV).clamp(-2, 2) * size * 4).half()
+    assert torch.isfinite(x).all()
+    _close(ops.int4_linear(x, packed, scales, block), x, w)
+    big = (torch.randn(m, 1024, generator=g, device=DEV).clamp(-2, 2) * 32752).half()      # up to 65504
+    small = w / 4096                                                                       # the same codes, smaller weights
+    _close(ops.int4_linear(big, packed, (scales.float() * 4096).half(), block), big, small)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
