@@ -1178,7 +1178,7 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
             raise ValueError(f"b200q: bias must have {n} elements")
         bias = bias.detach().to(dtype).contiguous()
         bias_at = bias.data_ptr()
-    packed, scales = _prep(packed), scales.contiguous()
+    packed, scales = _prep(packed), _prep(scales, 2)
     x2 = x if len(shape) == 2 else x.reshape(-1, k)
     xs, inner = x2.stride()
     if inner != 1 or (x2.data_ptr() | 2 * xs) & 15:

@@ -126,6 +126,18 @@ def test_bias_shapes_and_strides():
     assert torch.equal(ops.nvfp4_linear(x, shifted, scales, s2, bias), want)
 
 
+@pytest.mark.parametrize("block", [16, 32])
+def test_scales_at_odd_addresses(block):
+    from b200q import ops
+
+    packed, scales, s2, _ = _nvfp4(20, 96, torch.bfloat16, seed=3, block=block)
+    x = _x(3, 96, torch.bfloat16)
+    odd = torch.empty(scales.numel() + 1, dtype=torch.uint8, device=DEV)[1:]
+    odd.copy_(scales.view(torch.uint8).flatten())
+    want = ops.nvfp4_linear(x, packed, scales, s2, block=block)
+    assert torch.equal(ops.nvfp4_linear(x, packed, odd.view(torch.float8_e4m3fn).view(20, -1), s2, block=block), want)
+
+
 @pytest.mark.parametrize("scale", [1e-36, 1e-5, 1e5, 1e36])
 def test_bf16_rows_of_any_magnitude(scale):
     from b200q import ops
