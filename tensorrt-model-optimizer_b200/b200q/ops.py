@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from . import _cabi
-from ._cabi import call
+from ._cabi import B200QError, call, lib
 
 _DT = {torch.float32: _cabi.F32, torch.float16: _cabi.F16, torch.bfloat16: _cabi.BF16}
 
@@ -911,12 +911,12 @@ class KvStep(NamedTuple):
 def _launch(name: str, device: torch.device, *args) -> None:
     """``call`` on torch's current stream of ``device`` (the last argument of the entry point)."""
     index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if index == torch._C._cuda_getDevice():
-        call(name, *args, stream)
-    else:
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            call(name, *args, stream)
+            return _launch(name, device, *args)
+    status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        raise B200QError(name, status)
 
 
 def _int32_vector(t: torch.Tensor, what: str, device=None) -> int:
@@ -1132,17 +1132,26 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
 
 def int4_linear_supported(x: torch.Tensor, k: int, block: int) -> bool:
     """Whether ``int4_linear`` covers x [..., k] with groups of ``block``."""
-    return _w4_covers(x, k, block) and (block in (32, 64) or block % 128 == 0)
+    return _w4_covers(x, k) and _int4_sizes(k, block)
 
 
 def nvfp4_linear_supported(x: torch.Tensor, k: int, block: int = 16) -> bool:
     """Whether ``nvfp4_linear`` covers x [..., k] with scale blocks of ``block``."""
-    return _w4_covers(x, k, block) and block in (16, 32)
+    return _w4_covers(x, k) and _nvfp4_sizes(k, block)
 
 
-def _w4_covers(x: torch.Tensor, k: int, block: int) -> bool:
-    return (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1 and x.shape[-1] == k
-            and k % 32 == 0 and block > 0 and k % block == 0 and _w4_max_rows(k) > 0)
+def _w4_covers(x: torch.Tensor, k: int) -> bool:
+    return x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1 and x.shape[-1] == k
+
+
+@functools.lru_cache(maxsize=4096)
+def _int4_sizes(k: int, block: int) -> bool:
+    return block > 0 and (block in (32, 64) or block % 128 == 0) and k % 32 == 0 and k % block == 0 and _w4_max_rows(k) > 0
+
+
+@functools.lru_cache(maxsize=4096)
+def _nvfp4_sizes(k: int, block: int) -> bool:
+    return block in (16, 32) and k % 32 == 0 and _w4_max_rows(k) > 0
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1155,7 +1164,7 @@ def _w4_workspace(device: int, rows: int, n: int, k: int, int4_block: int) -> in
     return call("b200q_w4_linear_workspace", rows, n, k, int4_block)
 
 
-def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, covers, int4_block: int,
+def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, block: int, sizes, int4_block: int,
                scale2, bias):
     if not (x.is_cuda and packed.is_cuda and scales.is_cuda):
         _cuda(x, "x"), _cuda(packed, "packed"), _cuda(scales, "scales")
@@ -1166,7 +1175,7 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
         raise ValueError("b200q: packed must be [n, k/2] bytes")
     n, k = packed.shape
     k *= 2
-    if n == 0 or not covers(x, k, block):
+    if n == 0 or not shape or shape[-1] != k or not sizes(k, block):
         raise ValueError(f"b200q: no 4-bit product for x {tuple(shape)}, weight [{n}, {k}], block {block}")
     if scales.numel() != n * (k // block):
         raise ValueError(f"b200q: expected {n * (k // block)} scales, got {scales.numel()}")
@@ -1176,24 +1185,31 @@ def _w4_linear(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torch.T
     if bias is not None:
         if bias.numel() != n:
             raise ValueError(f"b200q: bias must have {n} elements")
-        bias = bias.detach().to(dtype).contiguous()
+        if bias.dtype is not dtype or not bias.is_contiguous():
+            bias = bias.detach().to(dtype).contiguous()
         bias_at = bias.data_ptr()
-    packed, scales = _prep(packed), _prep(scales, 2)
+    packed_at, scales_at = packed.data_ptr(), scales.data_ptr()
+    if packed_at & 15 or scales_at & 1 or not (packed.is_contiguous() and scales.is_contiguous()):
+        packed, scales = _prep(packed), _prep(scales, 2)
+        packed_at, scales_at = packed.data_ptr(), scales.data_ptr()
     x2 = x if len(shape) == 2 else x.reshape(-1, k)
     xs, inner = x2.stride()
-    if inner != 1 or (x2.data_ptr() | 2 * xs) & 15:
+    x_at = x2.data_ptr()
+    if inner != 1 or (x_at | 2 * xs) & 15:
         x2 = x2.clone(memory_format=torch.contiguous_format)
-        xs = k
+        xs, x_at = k, x2.data_ptr()
     m = x2.shape[0]
     out = torch.empty(*shape[:-1], n, dtype=dtype, device=dev)
-    most, x_at, out_at = _w4_max_rows(k), x2.data_ptr(), out.data_ptr()
+    most, out_at = _w4_max_rows(k), out.data_ptr()
+    status = _QGEMM_STATUS.get(dev)
+    status_at = (qgemm_status(dev) if status is None else status).data_ptr()
     extra = (block,) if scale2 is None else (block, scale2.data_ptr())
     for r in range(0, m, most):
         rows = min(most, m - r)
         need = _w4_workspace(dev.index, rows, n, k, int4_block)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None        # this call's own
-        _launch(name, dev, x_at + 2 * r * xs, xs, _DT[dtype], packed.data_ptr(), scales.data_ptr(), *extra, bias_at,
-                out_at + 2 * r * n, n, rows, n, k, ws.data_ptr() if need else None, need, qgemm_status(dev).data_ptr())
+        _launch(name, dev, x_at + 2 * r * xs, xs, _DT[dtype], packed_at, scales_at, *extra, bias_at,
+                out_at + 2 * r * n, n, rows, n, k, ws.data_ptr() if need else None, need, status_at)
     return out
 
 
@@ -1205,7 +1221,7 @@ def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, blo
     batches; a long prompt is faster through ``int4_dequantize`` and a GEMM."""
     if scales.dtype != x.dtype:
         raise TypeError(f"b200q: int4_linear takes scales of x's dtype {x.dtype}, got {scales.dtype}")
-    return _w4_linear("b200q_int4_linear", x, packed, scales, block, int4_linear_supported, block, None, bias)
+    return _w4_linear("b200q_int4_linear", x, packed, scales, block, _int4_sizes, block, None, bias)
 
 
 def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, scale2: torch.Tensor,
@@ -1217,4 +1233,4 @@ def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, sc
         raise TypeError("b200q: nvfp4_linear takes float8_e4m3fn scales")
     _cuda(x, "x")
     s2 = _kv_scale2(scale2, x.device)
-    return _w4_linear("b200q_nvfp4_linear", x, packed, scales, block, nvfp4_linear_supported, 0, s2, bias)
+    return _w4_linear("b200q_nvfp4_linear", x, packed, scales, block, _nvfp4_sizes, 0, s2, bias)
