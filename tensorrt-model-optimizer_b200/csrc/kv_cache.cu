@@ -212,9 +212,10 @@ extern "C" int b200q_kv_step(const int* lens, const int* new_lens, const int* fr
                              int* table, int64_t table_stride, int width, int requests, int page, int tokens,
                              int64_t* slots, int* positions, int* cu_new, int* lens_out, int* taken_out, int* status,
                              void* stream) {
-  B200Q_REQUIRE_PTR(lens); B200Q_REQUIRE_PTR(new_lens); B200Q_REQUIRE_PTR(taken); B200Q_REQUIRE_PTR(table);
+  B200Q_REQUIRE_PTR(lens); B200Q_REQUIRE_PTR(new_lens); B200Q_REQUIRE_PTR(taken);
   B200Q_REQUIRE_PTR(cu_new); B200Q_REQUIRE_PTR(lens_out); B200Q_REQUIRE_PTR(taken_out); B200Q_REQUIRE_PTR(status);
   if (nfree > 0) B200Q_REQUIRE_PTR(free_pages);
+  if (width > 0) B200Q_REQUIRE_PTR(table);
   if (tokens > 0) { B200Q_REQUIRE_PTR(slots); B200Q_REQUIRE_PTR(positions); }
   if (requests <= 0 || page <= 0 || tokens < 0 || nfree < 0 || width < 0 || table_stride < width) return B200Q_ERR_SHAPE;
   if (requests > kStepMaxRequests || tokens > (1 << 30)) return B200Q_ERR_UNSUPPORTED;

@@ -188,6 +188,21 @@ def test_append_of_nothing_and_of_unaligned_views():
     assert torch.equal(got, ops.nvfp4_dequantize(packed, scales, s2, torch.float16))
 
 
+def test_empty_tables_and_lists():
+    """A table without columns and an empty free list: every request with tokens is refused, none sees anything."""
+    from b200q import ops
+
+    table = torch.zeros(2, 0, dtype=torch.int32, device=DEV)
+    st = ops.kv_step(_i32([3, 0]), _i32([1, 0]), _i32([]), _i32([0]), table, 16, 2)
+    assert st.slots.tolist() == [-1, -1] and int(st.status) == 2 and st.lens.tolist() == [3, 0] and int(st.taken) == 0
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    kc, vc, s2 = _cache(1, 1, 16, 64), _cache(1, 1, 16, 64), torch.tensor(0.1, device=DEV)
+    out, lse = ops.nvfp4_kv_attention(q, kc, vc, s2, s2, table, _i32([5, 0]), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = ops.nvfp4_kv_attention(q, kc, vc, s2, s2, table, _i32([5, 0]), cu_q=_i32([1, 1, 1]), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()              # no request has a row
+
+
 # ------------------------------------------------------------------------------ attention ----
 
 def _dequantised(cache, s2):
