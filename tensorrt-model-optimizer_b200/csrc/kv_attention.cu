@@ -325,6 +325,7 @@ kv_attention_kernel(const AttnArgs a) {
     p_slot = p_slot + 1 == ST ? 0 : p_slot + 1;
     p_tok += kTile;
     if (--p_left > 0 && p_tok >= p_end && (p_left -= kSegCost) > 0) {
+      __syncwarp();                                 // every lane has read the segment that lane 0 now replaces
       if (lane == 0) next_segment<RT>(a, pc);
       __syncwarp();
       p_tok = warp * kStep;

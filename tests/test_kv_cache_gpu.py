@@ -637,3 +637,25 @@ def test_operators_refuse_what_they_do_not_cover():
     many = torch.zeros(8193, dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError):
         ops.kv_step(many, many, one, one, torch.zeros(8193, 1, dtype=torch.int32, device=DEV), 16, 1)
+
+
+# ------------------------------------------------------------------- segments of a single tile ----
+
+@pytest.mark.parametrize("dim,page,several", [(64, 16, False), (128, 64, False), (128, 48, True), (256, 32, True)])
+def test_attention_shares_that_begin_with_requests_of_one_tile(dim, page, several):
+    """Requests of at most one tile (128 tokens): a block handles several segments, and its two fetches ahead already
+    lie in different ones.  A segment of one tile is never split, so each request alone gives the same bits."""
+    from b200q import ops
+
+    lens = [1 + (37 * i) % 128 for i in range(600)]
+    q_lens = [1 + i % 3 if several else 1 for i in range(600)]
+    q, kc, vc, k2, v2, table, ln, cu = _attention_case(lens, q_lens, 3, 2, dim, page, torch.bfloat16, seed=page)
+    out, lse = ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, ln, cu_q=cu if several else None, return_lse=True)
+    for _ in range(3):
+        assert torch.equal(ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, ln, cu_q=cu if several else None), out)
+    first = cu.tolist()
+    for b in range(0, 600, 7):
+        rows = slice(first[b], first[b + 1])
+        alone, alse = ops.nvfp4_kv_attention(q[rows], kc, vc, k2, v2, table[b:b + 1], ln[b:b + 1],
+                                             cu_q=_i32([0, q_lens[b]]) if several else None, return_lse=True)
+        assert torch.equal(alone, out[rows]) and torch.equal(alse, lse[rows])
