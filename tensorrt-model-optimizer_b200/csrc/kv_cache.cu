@@ -221,7 +221,8 @@ extern "C" int b200q_kv_step(const int* lens, const int* new_lens, const int* fr
   if (requests > kStepMaxRequests || tokens > (1 << 30)) return B200Q_ERR_UNSUPPORTED;
   const size_t smem = sizeof(int) * (3 * static_cast<size_t>(requests) + 2);
   static std::atomic<uint64_t> done;
-  if (smem > 48 * 1024 && !allow_smem(reinterpret_cast<const void*>(kv_step_kernel), 3 * sizeof(int) * (kStepMaxRequests + 1), done))
+  // the 48 KB of the default limit hold the kernel's static words too (1 KB is more than they take)
+  if (smem > 47 * 1024 && !allow_smem(reinterpret_cast<const void*>(kv_step_kernel), 3 * sizeof(int) * (kStepMaxRequests + 1), done))
     return B200Q_ERR_CUDA;
   const int grid = grid_for(static_cast<int64_t>(tokens) + requests, 4 * kStepThreads, 1);
   launch_pdl(kv_step_kernel, grid, kStepThreads, smem, static_cast<cudaStream_t>(stream), lens, new_lens, free_pages, nfree,

@@ -659,3 +659,29 @@ def test_attention_shares_that_begin_with_requests_of_one_tile(dim, page, severa
         alone, alse = ops.nvfp4_kv_attention(q[rows], kc, vc, k2, v2, table[b:b + 1], ln[b:b + 1],
                                              cu_q=_i32([0, q_lens[b]]) if several else None, return_lse=True)
         assert torch.equal(alone, out[rows]) and torch.equal(alse, lse[rows])
+
+
+def test_step_numbers_of_requests_around_the_default_shared_memory():
+    """The scans of 4090 to 4095 requests fit the 48 KB a kernel has by default only without its own 72 bytes.  In a
+    process of its own, the smaller numbers first: a larger call raises the limit for the rest of the process."""
+    import subprocess
+    import sys
+
+    code = """
+import sys
+sys.path[:0] = %r
+import torch
+from b200q import ops
+for b in (4089, 4090, 4092, 4095, 4096, 4097):
+    lens = torch.arange(b, dtype=torch.int32, device="cuda") %% 5
+    one = torch.ones(b, dtype=torch.int32, device="cuda")
+    table = torch.full((b, 1), -1, dtype=torch.int32, device="cuda")
+    free = torch.arange(b, dtype=torch.int32, device="cuda").flip(0)
+    held = lens > 0
+    table[held, 0] = free[:int(held.sum())]
+    st = ops.kv_step(lens, one, free, held.sum().int().view(1), table, 16, b)
+    assert int(st.status) == 0 and int(st.taken) == b and torch.equal(st.lens, lens + 1), b
+    assert torch.equal(st.slots, table[:, 0].long() * 16 + lens) and sorted(table[:, 0].tolist()) == list(range(b)), b
+""" % sys.path
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
