@@ -256,3 +256,56 @@ def test_refusals():
         ops.nvfp4_linear(x, packed, scales.view(-1).view(torch.uint8)[: 16 * 4], torch.ones((), device=DEV), block=64)
     assert not ops.nvfp4_linear_supported(x[:, :16], 16, 16) and not ops.int4_linear_supported(x, 256, 16)
     assert ops.nvfp4_linear_supported(x, 256, 32) and ops.int4_linear_supported(x, 256, 256)
+
+
+# ------------------------------------------------------- several tiles a CTA, sums that leave no room ----
+
+# (rows, n, k) whose CTAs walk over several tiles on 148 SMs: with K whole, over the warps of a tile, over CTAs, and over both
+WALKS = [(1, 40003, 256), (1, 40003, 640), (1, 40003, 2304), (8, 8203, 6400), (9, 4099, 2688), (9, 40003, 1024),
+         (9, 4099, 12672), (16, 4099, 5632), (17, 4099, 3584), (32, 40003, 256), (32, 4099, 2304), (32, 4099, 5632)]
+
+
+FORMATS = [("int4", 32), ("int4", 64), ("int4", 128), ("int4", 256), ("nvfp4", 16), ("nvfp4", 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k,fmt,block", [w + f for w in WALKS for f in FORMATS if w[2] % f[1] == 0])
+def test_ctas_that_walk_over_several_tiles(m, n, k, fmt, block, dtype):
+    """x holds small integers, so that every sum of 128 elements (INT4: of a group where that is less) is exact in fp32:
+    INT4 adds integers, NVFP4 multiples of 2^-5 below 2^7.  What is left is counted from those sums S: each is off by
+    3 * 2^-24 (reciprocal or scale2, product), and the additions that follow (INT4: one for each S; in either format the
+    joins of at most 16 warps and 16 CTAs) by 2^-24 each of at most the sum of |S|.  NVFP4's chain over a warp's elements
+    stays exact: partial sums below 2^17, multiples of 2^-5.  Weights rounded to 16 bits would be off by far more.  The
+    reference's own 64 bits count too, where a sum cancels: k products and additions of 2^-53 of the sum of magnitudes."""
+    from b200q import ops
+
+    g = torch.Generator(device=DEV).manual_seed(m + n + k)
+    x = torch.randint(-4, 5, (m, k), generator=g, device=DEV).to(dtype)
+    packed = torch.randint(0, 256, (n, k // 2), generator=g, device=DEV).to(torch.uint8)
+    if fmt == "int4":
+        scales = (torch.rand(n * (k // block), 1, generator=g, device=DEV) * 180 + 20).to(dtype)
+        out = ops.int4_linear(x, packed, scales, block)
+    else:
+        s2 = torch.tensor(0.00123, device=DEV)
+        scales = torch.randint(0x30, 0x49, (n, k // block), generator=g, device=DEV).to(torch.uint8).view(torch.float8_e4m3fn)
+        out = ops.nvfp4_linear(x, packed, scales, s2, block=block)
+    unit = min(block, 128) if fmt == "int4" else 128
+    adds = (k // unit if fmt == "int4" else 0) + 40
+    lut = torch.tensor(E2M1, dtype=torch.float64, device=DEV)
+    xg = x.double().unflatten(1, (-1, unit)).transpose(0, 1)               # [groups, m, unit]
+    for at in range(0, n, 4096):
+        c = packed[at:at + 4096]
+        if fmt == "int4":
+            w = (torch.stack((c >> 4, c & 15), -1).reshape(c.shape[0], -1, block).double() - 8) / scales.view(n, -1, 1)[at:at + 4096].double()
+        else:
+            w = lut[torch.stack((c & 15, c >> 4), -1).reshape(c.shape[0], -1, block).long()]
+            w = w * scales[at:at + 4096].float().double().unsqueeze(-1) * s2.double()
+        w = w.reshape(c.shape[0], -1, unit).permute(1, 2, 0)               # [groups, unit, n]
+        parts = xg @ w
+        ref, size = parts.sum(0), parts.abs().sum(0)
+        own = (k + 2) * 2.0 ** -53 * (xg.abs() @ w.abs()).sum(0)
+        got = out[:, at:at + 4096].double()
+        info = torch.finfo(dtype)
+        top = torch.maximum(ref.abs(), got.abs()).clamp(min=info.tiny)
+        half = torch.exp2(torch.floor(torch.log2(top))) * info.eps / 2
+        assert float(((got - ref).abs() - half - size * adds * 2.0 ** -24 - own).max()) <= 0
