@@ -526,8 +526,8 @@ int b200q_nvfp4_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_
  * multiples of 8; last dimension contiguous); out contiguous of type T; lse [tokens, heads * group] fp32 (natural
  * logarithm) or NULL.  dim 64, 128 or 256; page a multiple of 16; table rows as in b200q_kv_step (an id outside
  * [0, pages) hides its tokens; lens beyond width * page are cut).  cu_q is non-decreasing; rows of q in front of
- * cu_q[0] and from cu_q[requests] on are not computed: their output is left as it is, or zeroed (lse -inf) where
- * zero_tail != 0.  out must not overlap q.
+ * cu_q[0] and from cu_q[requests] on are not computed: with zero_tail 0 their output and lse are left as they are,
+ * with 1 they are zero and -inf, with 2 lse is -inf and out is left as it is.  out must not overlap q.
  * workspace: b200q_nvfp4_kv_attention_workspace(...) bytes, this call's alone until it has run.  Lengths are read on the
  * device only: the call can be captured and replayed with others.  width * page and
  * heads * page at most 2^30. */

@@ -95,7 +95,7 @@ class NVFP4KVCache:
     def attend(self, layer: int, q: torch.Tensor, step: ops.KvStep, scale: float | None = None, out=None,
                return_lse: bool = False):
         """Causal attention of the step's queries [tokens, heads, head_dim] over ``layer`` (``ops.nvfp4_kv_attention``);
-        rows behind the last request's are zero."""
+        rows behind the last request's are zero (a given ``out`` keeps what it holds there)."""
         kc, vc, k2, v2 = self.layers[layer]
         return ops.nvfp4_kv_attention(q, kc, vc, k2, v2, self.block_table, step.lens, cu_q=step.cu_new, scale=scale, out=out,
                                       return_lse=return_lse)

@@ -1076,7 +1076,8 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
     ``lens`` int32 [requests]: tokens of each request in the cache, the step's own included; ``block_table`` int32
     [requests, width].  Without ``cu_q`` every request has one query; with it (int32 [requests + 1], not decreasing)
     request b owns rows cu_q[b] : cu_q[b + 1], its last tokens, each seeing everything up to itself.  Rows that see nothing are
-    zero (lse -inf), and so are rows behind the last request unless ``out`` is given, which keeps them.  ``scale``
+    zero (lse -inf), and so are rows in front of the first and behind the last request; a given ``out`` keeps what it holds
+    there (their lse is -inf all the same).  ``scale``
     defaults to dim ** -0.5.  Lengths are read on the device: a captured call serves later lengths too."""
     if not q.is_cuda:
         _cuda(q, "q")
@@ -1124,7 +1125,7 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
             vc.data_ptr(), vs.data_ptr(), k2.data_ptr(), v2.data_ptr(), block_table.data_ptr(), stride, width, lens.data_ptr(),
             cu_q.data_ptr() if cu_q is not None else None, b, tokens, heads, group, dim, pages, page,
             dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr() if return_lse else None,
-            int(zero_tail), ws.data_ptr(), need)
+            1 if zero_tail else 2 if return_lse else 0, ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 

@@ -60,7 +60,8 @@ struct AttnArgs {
   float2* part_ml;                                  // [ctas, 2, rows]
   int4* desc;                                       // [ctas][2]: pieces, first query, kv head, first row; rows
   FastDiv chunks_per_page, group_div;
-  int width, requests, tokens, heads, group, page, pages, zero_tail;
+  int width, requests, tokens, heads, group, page, pages;
+  int zero_tail;                                    // rows of no request: 0 left as they are, 1 zero and lse -inf, 2 lse only
   float scale;
 };
 
@@ -734,7 +735,8 @@ kv_merge_kernel(const AttnArgs a) {
     const int64_t end = head + static_cast<int64_t>(a.tokens) * heads - tail, nb = static_cast<int64_t>(gridDim.x) * gridDim.y;
     for (int64_t i = blockIdx.y * gridDim.x + blockIdx.x; i < end; i += nb) {
       const int64_t r = i < head ? i : tail + i - head;
-      for (int d = threadIdx.x; d < D; d += 128) static_cast<T*>(a.out)[r * D + d] = Elem<T>::from_float(0.f);
+      if (a.zero_tail != 2)
+        for (int d = threadIdx.x; d < D; d += 128) static_cast<T*>(a.out)[r * D + d] = Elem<T>::from_float(0.f);
       if (a.lse && threadIdx.x == 0) a.lse[r] = -INFINITY;
     }
   }

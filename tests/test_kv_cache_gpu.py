@@ -685,3 +685,19 @@ for b in (4089, 4090, 4092, 4095, 4096, 4097):
 """ % sys.path
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_log_sums_of_rows_without_a_request_when_out_is_given():
+    """``out`` keeps its rows in front of the first request and behind the last one; the log-sums are a fresh buffer and
+    say -inf there, whatever its memory held before."""
+    from b200q import ops
+
+    q, kc, vc, k2, v2, table, ln, cu = _attention_case([40, 21], [3, 2], 1, 4, 64, 16, torch.bfloat16)
+    want, wlse = ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, ln, cu_q=cu, return_lse=True)
+    qp = torch.cat([q.new_full((3, 4, 64), math.nan), q, q.new_full((4, 4, 64), math.nan)])
+    for _ in range(3):
+        torch.full((12, 4), 3.0, dtype=torch.float32, device=DEV)              # freed memory that is no -inf
+        buf = torch.full_like(qp, 7)
+        out, lse = ops.nvfp4_kv_attention(qp, kc, vc, k2, v2, table, ln, cu_q=cu + 3, out=buf, return_lse=True)
+        assert out is buf and torch.equal(buf[3:8], want) and (buf[:3] == 7).all() and (buf[8:] == 7).all()
+        assert torch.equal(lse[3:8], wlse) and (lse[:3] == -math.inf).all() and (lse[8:] == -math.inf).all()
