@@ -500,10 +500,15 @@ int64_t b200q_w4_linear_workspace(int rows, int64_t n, int64_t k, int int4_block
  * 1 (free list exhausted: this request and the later ones that need a page), 2 (wider than its table row),
  * 4 (negative or too large a length), 8 (more new tokens than rows).  lens_out and taken_out must not
  * overlap the inputs; the call may be repeated on the same inputs.  At most 8192 requests.  Pointers need
- * their element's alignment only. */
+ * their element's alignment only.
+ * b200q_kv_step_seen also writes seen[b] (NULL: not), the length to attend with: lens_out[b], or 0 for a refused
+ * request, whose rows cu_new still counts and whose keys are not in the cache. */
 int b200q_kv_step(const int* lens, const int* new_lens, const int* free_pages, int nfree, const int* taken, int* table,
                   int64_t table_stride, int width, int requests, int page, int tokens, int64_t* slots, int* positions,
                   int* cu_new, int* lens_out, int* taken_out, int* status, void* stream);
+int b200q_kv_step_seen(const int* lens, const int* new_lens, const int* free_pages, int nfree, const int* taken, int* table,
+                       int64_t table_stride, int width, int requests, int page, int tokens, int64_t* slots,
+                       int* positions, int* cu_new, int* lens_out, int* taken_out, int* status, int* seen, void* stream);
 
 /* New keys and values quantised to NVFP4 and written at their slots.  k, v: [tokens, heads, dim] of type T with
  * the given strides in elements (last dimension contiguous; pointers and strides multiples of 32 bytes), dim a

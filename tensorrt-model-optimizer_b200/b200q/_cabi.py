@@ -81,6 +81,7 @@ SIGNATURES = {
     "b200q_hadamard": [_p, _p, _i64, _i, _i, _f, _p],
     "b200q_mx_fake": [_p, _p, _i64, _i, _i, _i, _p],
     "b200q_kv_step": [_p, _p, _p, _i, _p, _p, _i64, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p],
+    "b200q_kv_step_seen": [_p, _p, _p, _i, _p, _p, _i64, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p],
     "b200q_nvfp4_kv_append": [_p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p, _i, _i, _p, _p,
                               _p],
     "b200q_nvfp4_kv_attention": [_p, _i64, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _i, _i,

@@ -79,8 +79,8 @@ class NVFP4KVCache:
 
     def step(self, new_lens: torch.Tensor, tokens: int) -> ops.KvStep:
         """Room for ``new_lens[r]`` more tokens of every request r (int32 [max_requests], 0 for rows without any), in
-        ``tokens`` rows of the step's tensors.  Lengths and tables advance; a request that does not fit keeps its length
-        and gets no slots (see ``check``)."""
+        ``tokens`` rows of the step's tensors.  Lengths and tables advance; a request that does not fit keeps its length,
+        gets no slots, and its rows see nothing (see ``check``)."""
         st = ops.kv_step(self.lens, new_lens, self.free_pages, self.taken, self.block_table, self.page_size, tokens)
         self.lens.copy_(st.lens)
         self.taken.copy_(st.taken)
@@ -95,9 +95,11 @@ class NVFP4KVCache:
     def attend(self, layer: int, q: torch.Tensor, step: ops.KvStep, scale: float | None = None, out=None,
                return_lse: bool = False):
         """Causal attention of the step's queries [tokens, heads, head_dim] over ``layer`` (``ops.nvfp4_kv_attention``);
-        rows behind the last request's are zero (a given ``out`` keeps what it holds there)."""
+        rows of a request that the step refused are zero, and so are rows behind the last request's (a given ``out`` keeps
+        what it holds there)."""
         kc, vc, k2, v2 = self.layers[layer]
-        return ops.nvfp4_kv_attention(q, kc, vc, k2, v2, self.block_table, step.lens, cu_q=step.cu_new, scale=scale, out=out,
+        lens = step.lens if step.seen is None else step.seen
+        return ops.nvfp4_kv_attention(q, kc, vc, k2, v2, self.block_table, lens, cu_q=step.cu_new, scale=scale, out=out,
                                       return_lse=return_lse)
 
     def release(self, request: int) -> None:

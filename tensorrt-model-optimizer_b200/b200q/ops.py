@@ -892,17 +892,24 @@ def nvfp4_gemm(a4: torch.Tensor, sfa: torch.Tensor, b4: torch.Tensor, sfb: torch
 
 # --------------------------------------------------------------------------- paged NVFP4 KV cache --
 
-class KvStep(NamedTuple):
-    """What ``kv_step`` returns (all on the device): ``slots`` int64 and ``positions`` int32 per token row,
-    ``cu_new`` int32 [requests + 1] first row of each request, ``lens`` int32 the lengths after the step,
-    ``taken`` int32 [1] free pages handed out so far, ``status`` int32 [1] (0 = every request was served)."""
-
+class _KvStepFields(NamedTuple):
     slots: torch.Tensor
     positions: torch.Tensor
     cu_new: torch.Tensor
     lens: torch.Tensor
     taken: torch.Tensor
     status: torch.Tensor
+
+
+class KvStep(_KvStepFields):
+    """What ``kv_step`` returns (all on the device): ``slots`` int64 and ``positions`` int32 per token row,
+    ``cu_new`` int32 [requests + 1] first row of each request, ``lens`` int32 the lengths after the step,
+    ``taken`` int32 [1] free pages handed out so far, ``status`` int32 [1] (0 = every request was served).
+
+    Beside these six, ``seen`` int32 [requests] holds the lengths to attend with: ``lens``, but 0 for a refused request,
+    whose rows have no keys in the cache."""
+
+    seen: torch.Tensor | None = None
 
 
 # The wrappers below run once or several times a layer of every decoding step, on kernels of a few microseconds:
@@ -951,7 +958,8 @@ def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor
     int32 holds its page ids and receives the new ones IN PLACE, taken in request order from
     ``free_pages[taken:]``.  ``tokens`` is the number of token rows of the step's tensors; rows behind the
     last request get slot -1.  A request that does not fit (free list, table row, rows, a negative length)
-    is refused: it keeps its length, its rows get slot -1, and ``status`` is not zero (bits 1, 2, 8, 4).
+    is refused: it keeps its length, its rows get slot -1, and ``status`` is not zero (bits 1, 2, 8, 4).  The step's
+    attention takes ``seen`` for its lengths, so that a refused request's rows see nothing.
     The inputs other than the table stay as they are; repeating the call gives the same result."""
     b = _int32_vector(lens, "lens")
     dev = lens.device
@@ -964,13 +972,15 @@ def kv_step(lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor
     if stride < width:
         raise ValueError("b200q: the rows of block_table overlap")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    ints = torch.empty(2 * b + 3 + tokens, dtype=torch.int32, device=dev)
+    ints = torch.empty(3 * b + 3 + tokens, dtype=torch.int32, device=dev)
     at = ints.data_ptr()
-    _launch("b200q_kv_step", dev, lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), nfree, taken.data_ptr(),
-            block_table.data_ptr(), stride, width, b, page_size, tokens, slots.data_ptr(), at + 8 * b + 12, at, at + 4 * b + 4,
-            at + 8 * b + 4, at + 8 * b + 8)
-    cu, lens_out, taken_out, status, positions = ints.split_with_sizes((b + 1, b, 1, 1, tokens))
-    return KvStep(slots, positions, cu, lens_out, taken_out, status)
+    _launch("b200q_kv_step_seen", dev, lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), nfree, taken.data_ptr(),
+            block_table.data_ptr(), stride, width, b, page_size, tokens, slots.data_ptr(), at + 12 * b + 12, at, at + 4 * b + 4,
+            at + 8 * b + 4, at + 8 * b + 8, at + 8 * b + 12)
+    cu, lens_out, taken_out, status, seen, positions = ints.split_with_sizes((b + 1, b, 1, 1, b, tokens))
+    step = KvStep(slots, positions, cu, lens_out, taken_out, status)
+    step.seen = seen
+    return step
 
 
 def _kv_pages(cache, what: str, device):

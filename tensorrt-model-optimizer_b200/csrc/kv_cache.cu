@@ -13,7 +13,8 @@ namespace b200q {
 //   base = taken + exclusive scan of need,   table[b, have + i] = free[base + i]
 //   cu   = exclusive scan of n,              token t of b: pos = L + t - cu[b], slot = table[b, pos/p]*p + pos%p
 // A request that is malformed, wider than its table row or beyond the free list is refused: it keeps its
-// length, its tokens get slot -1, and a status bit says why.
+// length, its tokens get slot -1, and a status bit says why.  Its rows have no keys in the cache, so `seen`, the length
+// that the step's attention takes, is 0 for it.
 //
 // One launch and no order between blocks: every block repeats the two scans in shared memory (4 words a
 // request), then writes its share of the table entries and of the token rows, each found by a binary search
@@ -63,7 +64,7 @@ kv_step_kernel(const int* __restrict__ lens, const int* __restrict__ new_lens, c
                int nfree, const int* __restrict__ taken_in, int* __restrict__ table, int64_t table_stride, int width,
                int requests, int page, int tokens, int64_t* __restrict__ slots, int* __restrict__ positions,
                int* __restrict__ cu_out, int* __restrict__ lens_out, int* __restrict__ taken_out,
-               int* __restrict__ status) {
+               int* __restrict__ status, int* __restrict__ seen) {
   extern __shared__ int step_smem[];
   int* cu = step_smem;                       // [requests + 1] first token row of a request, clamped to `tokens`
   int* base = cu + requests + 1;             // [requests + 1] first index into the free list, counted from `taken`
@@ -139,6 +140,7 @@ kv_step_kernel(const int* __restrict__ lens, const int* __restrict__ new_lens, c
   for (int r = first; r < requests; r += step) {
     cu_out[r] = cu[r];
     lens_out[r] = have[r] < 0 ? lens[r] : lens[r] + new_lens[r];
+    if (seen) seen[r] = have[r] < 0 ? 0 : lens[r] + new_lens[r];
   }
   if (first == 0) {
     cu_out[requests] = real;
@@ -208,10 +210,10 @@ kv_append_kernel(KvSide k, KvSide v, const int64_t* __restrict__ slots, int nblo
 
 using namespace b200q;
 
-extern "C" int b200q_kv_step(const int* lens, const int* new_lens, const int* free_pages, int nfree, const int* taken,
-                             int* table, int64_t table_stride, int width, int requests, int page, int tokens,
-                             int64_t* slots, int* positions, int* cu_new, int* lens_out, int* taken_out, int* status,
-                             void* stream) {
+extern "C" int b200q_kv_step_seen(const int* lens, const int* new_lens, const int* free_pages, int nfree, const int* taken,
+                                  int* table, int64_t table_stride, int width, int requests, int page, int tokens,
+                                  int64_t* slots, int* positions, int* cu_new, int* lens_out, int* taken_out, int* status,
+                                  int* seen, void* stream) {
   B200Q_REQUIRE_PTR(lens); B200Q_REQUIRE_PTR(new_lens); B200Q_REQUIRE_PTR(taken);
   B200Q_REQUIRE_PTR(cu_new); B200Q_REQUIRE_PTR(lens_out); B200Q_REQUIRE_PTR(taken_out); B200Q_REQUIRE_PTR(status);
   if (nfree > 0) B200Q_REQUIRE_PTR(free_pages);
@@ -226,8 +228,16 @@ extern "C" int b200q_kv_step(const int* lens, const int* new_lens, const int* fr
     return B200Q_ERR_CUDA;
   const int grid = grid_for(static_cast<int64_t>(tokens) + requests, 4 * kStepThreads, 1);
   launch_pdl(kv_step_kernel, grid, kStepThreads, smem, static_cast<cudaStream_t>(stream), lens, new_lens, free_pages, nfree,
-             taken, table, table_stride, width, requests, page, tokens, slots, positions, cu_new, lens_out, taken_out, status);
+             taken, table, table_stride, width, requests, page, tokens, slots, positions, cu_new, lens_out, taken_out, status, seen);
   return launch_status();
+}
+
+extern "C" int b200q_kv_step(const int* lens, const int* new_lens, const int* free_pages, int nfree, const int* taken,
+                             int* table, int64_t table_stride, int width, int requests, int page, int tokens,
+                             int64_t* slots, int* positions, int* cu_new, int* lens_out, int* taken_out, int* status,
+                             void* stream) {
+  return b200q_kv_step_seen(lens, new_lens, free_pages, nfree, taken, table, table_stride, width, requests, page, tokens, slots,
+                            positions, cu_new, lens_out, taken_out, status, nullptr, stream);
 }
 
 extern "C" int b200q_nvfp4_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,

@@ -701,3 +701,18 @@ def test_log_sums_of_rows_without_a_request_when_out_is_given():
         out, lse = ops.nvfp4_kv_attention(qp, kc, vc, k2, v2, table, ln, cu_q=cu + 3, out=buf, return_lse=True)
         assert out is buf and torch.equal(buf[3:8], want) and (buf[:3] == 7).all() and (buf[8:] == 7).all()
         assert torch.equal(lse[3:8], wlse) and (lse[:3] == -math.inf).all() and (lse[8:] == -math.inf).all()
+
+
+def test_step_says_what_a_request_sees():
+    """``seen``: the length after the step, 0 for a request that was refused, whatever the reason."""
+    from b200q import ops
+
+    lens, new = [5, -1, 30, 7, 3, 2 ** 31 - 2, 9, 4], [3, 4, 40, -2, 1, 5, 50, 0]
+    table = _i32([[0, -1, -1], [-1] * 3, [1, 2, -1], [3, -1, -1], [4, -1, -1], [-1] * 3, [5, -1, -1], [6, -1, -1]])
+    st = ops.kv_step(_i32(lens), _i32(new), _i32(list(range(7))), _i32([7]), table, 16, 60)
+    # 103 rows are asked for and 60 there: requests behind the end are refused, the last one, without any row, among them
+    assert len(st) == 6 and st.seen.tolist() == [8, 0, 0, 0, 4, 0, 0, 0]
+    st = ops.kv_step(_i32([16, 3, 16]), _i32([1, 1, 0]), _i32([0, 1, 2]), _i32([3]), _i32([[0, -1], [1, -1], [2, -1]]), 16, 2)
+    assert int(st.status) == 1 and st.seen.tolist() == [0, 4, 16]
+    st = ops.kv_step(_i32([5, 9, 2]), _i32([4, 4, 5]), _i32([0, 1, 2, 3]), _i32([3]), _i32([[0, -1], [1, -1], [2, -1]]), 16, 10)
+    assert int(st.status) == 8 and st.seen.tolist() == [9, 13, 0]

@@ -378,3 +378,42 @@ def test_decoding_step_of_a_4_bit_model():
         got = torch.cat(outs[r]).float()
         # the two differ by roundings to bf16 in between (a dozen of 2^-8 on values of the output's size)
         assert float((got - want).norm() / want.norm()) <= 12 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("refused", ["no page", "row full", "too few rows"])
+def test_rows_of_a_refused_request_see_nothing(refused):
+    """A refused request's rows have no keys of their own in the cache: they are zero with log-sum -inf, and the other
+    requests' rows are what they are without it."""
+    from b200q import ops
+
+    cache, _ = _cache(num_pages=4 if refused == "no page" else 24, max_pages_per_request=2 if refused == "row full" else 4)
+    g = torch.Generator(device=DEV).manual_seed(2)
+
+    def step(new, rows):
+        t = sum(new)
+        st = cache.step(_int32(new), rows)
+        q = torch.randn(t, 8, 64, generator=g, device=DEV).bfloat16()
+        k, v = (torch.randn(t, 2, 64, generator=g, device=DEV).bfloat16() for _ in range(2))
+        cache.append(0, k[:rows], v[:rows], st)
+        return q, st, cache.attend(0, q[:rows], st, return_lse=True)
+
+    first = [20, 30, 16] if refused != "no page" else [20, 16, 1]
+    step(first, sum(first))
+    cache.check()
+    held = cache.lens.tolist()
+    new = [1, 5, 2] if refused != "too few rows" else [1, 2, 5]
+    rows = sum(new) if refused != "too few rows" else sum(new) - 1
+    bad = 1 if refused != "too few rows" else 2
+    q, st, (out, lse) = step(new, rows)
+    with pytest.raises(RuntimeError):
+        cache.check()
+    assert cache.lens.tolist() == [n + (m if r != bad else 0) for r, (n, m) in enumerate(zip(held, new))]
+    rows_of = [slice(a, b) for a, b in zip(st.cu_new.tolist(), st.cu_new.tolist()[1:])]
+    assert (st.slots[rows_of[bad]] == -1).all()
+    assert (out[rows_of[bad]] == 0).all() and (lse[rows_of[bad]] == -float("inf")).all()
+    see = cache.lens.clone()
+    see[bad] = 0
+    kc, vc, k2, v2 = cache.layers[0]
+    want, wlse = ops.nvfp4_kv_attention(q[:rows], kc, vc, k2, v2, cache.block_table, see, cu_q=st.cu_new, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    assert all((lse[rows_of[r]] > -float("inf")).all() for r in range(3) if r != bad)
