@@ -35,32 +35,44 @@ def weight_only_gemm(quant_module, input_tensor, bias=None):
     return ops.nvfp4_linear(input_tensor, packed, wq._scale, wq._double_scale, bias, block)
 
 
-def _covered(module, input) -> bool:
-    """Whether the module's weight is packed in a layout that the products read, for inputs like ``input``."""
+def _layout_covered(module) -> bool:
+    """Whether the module's weight is packed in a layout that the products read: what lasts from call to call."""
     wq, weight = module.weight_quantizer, module.weight
-    if not isinstance(weight, QTensorWrapper) or not weight.data.is_cuda or not hasattr(wq, "_scale"):
+    if not isinstance(weight, QTensorWrapper) or not hasattr(wq, "_scale"):
         return False
     kind, shape, dtype = (weight.metadata[key] for key in ("qtensor_class", "shape", "dtype"))
-    if kind not in (INT4QTensor, NVFP4QTensor) or len(shape) != 2 or dtype != input.dtype or input.shape[-1] != shape[1]:
-        return False
-    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != dtype:   # F.linear would cast both
+    if kind not in (INT4QTensor, NVFP4QTensor) or len(shape) != 2 or dtype not in (torch.float16, torch.bfloat16):
         return False
     block = (getattr(wq, "block_sizes", None) or {}).get(-1)
     if not isinstance(block, int) or weight.data.numel() * 2 != shape[0] * shape[1]:      # padded rows
         return False
     if kind is INT4QTensor:
-        return wq._scale.dtype == input.dtype and ops.int4_linear_supported(input, shape[1], block)
-    return hasattr(wq, "_double_scale") and ops.nvfp4_linear_supported(input, shape[1], block)
+        return wq._scale.dtype == dtype and ops._int4_sizes(shape[1], block)
+    return hasattr(wq, "_double_scale") and ops._nvfp4_sizes(shape[1], block)
+
+
+def _covered(module, input) -> bool:
+    """Whether the products take this call: the weight's layout, and inputs and autocast as they are now."""
+    if not _layout_covered(module):
+        return False
+    weight = module.weight
+    shape, dtype = weight.metadata["shape"], weight.metadata["dtype"]
+    if not (weight.data.is_cuda and input.is_cuda) or dtype != input.dtype or input.shape[-1] != shape[1]:
+        return False
+    # F.linear would cast both
+    return not (torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != dtype)
 
 
 def _weight_only_availability_check(module, input, args, kwargs) -> bool:
+    """The answer is remembered by the layer, so nothing that changes from call to call may go into it: the products
+    look at the input themselves."""
     from ..nn import RealQuantLinear, TensorQuantizer
 
     if not (isinstance(module, RealQuantLinear) and isinstance(getattr(module, "input_quantizer", None), TensorQuantizer)
             and isinstance(getattr(module, "weight_quantizer", None), TensorQuantizer)):
         return False
     return (getattr(module, "_weight_only_gemm", False) and not module.input_quantizer.is_enabled
-            and module.weight_quantizer.is_enabled and torch.cuda.is_available() and input.is_cuda and _covered(module, input))
+            and module.weight_quantizer.is_enabled and _layout_covered(module))
 
 
 class WeightOnlyLinear(Function):

@@ -417,3 +417,30 @@ def test_rows_of_a_refused_request_see_nothing(refused):
     want, wlse = ops.nvfp4_kv_attention(q[:rows], kc, vc, k2, v2, cache.block_table, see, cu_q=st.cu_new, return_lse=True)
     assert torch.equal(out, want) and torch.equal(lse, wlse)
     assert all((lse[rows_of[r]] > -float("inf")).all() for r in range(3) if r != bad)
+
+
+@pytest.mark.parametrize("name", CFGS)
+def test_a_first_call_that_is_not_covered_is_not_remembered(name):
+    """A marked layer whose first call runs under autocast to another type, or with another input type, still reads the
+    packed weight in the calls that are covered."""
+    import b200q as mtq
+    from b200q import ops
+
+    x = torch.randn(4, 256, device=DEV, dtype=torch.float16)
+    want = _compressed(getattr(mtq, name), torch.float16, {"weight_only_gemm": True})(x)
+    calls, real = [], ops._w4_linear
+    try:
+        ops._w4_linear = lambda *a, **k: (calls.append(a[0]), real(*a, **k))[1]
+        model = _compressed(getattr(mtq, name), torch.float16, {"weight_only_gemm": True})
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert model(x).dtype == torch.bfloat16
+        assert not calls
+        assert torch.equal(model(x), want) and len(calls) == 2
+        calls.clear()
+        model = _compressed(getattr(mtq, name), torch.float16, {"weight_only_gemm": True})
+        with pytest.raises(RuntimeError):
+            model(x.float())                                 # as F.linear says it of two types
+        assert not calls
+        assert torch.equal(model(x), want) and len(calls) == 2
+    finally:
+        ops._w4_linear = real
