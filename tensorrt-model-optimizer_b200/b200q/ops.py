@@ -1076,6 +1076,15 @@ def nvfp4_kv_attention_supported(q: torch.Tensor, heads: int, page: int) -> bool
             and heads > 0 and q.shape[1] > 0 and q.shape[1] % heads == 0 and page > 0 and page % 16 == 0)
 
 
+def _spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the addresses from a's first to its last element and b's have one in common."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    first, last = zip(*((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+                        for t in (a, b)))
+    return first[0] < last[1] and first[1] < last[0]
+
+
 def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor, v_scale2: torch.Tensor,
                        block_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor | None = None,
                        scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
@@ -1117,7 +1126,7 @@ def nvfp4_kv_attention(q: torch.Tensor, k_cache, v_cache, k_scale2: torch.Tensor
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("b200q: out must be a contiguous, 16-byte aligned tensor like q")
-    elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+    elif _spans_overlap(out, q):
         raise ValueError("b200q: out must not share q's memory")
     lse = torch.empty(tokens, qheads, dtype=torch.float32, device=dev) if return_lse else None
     if b == 0 or tokens == 0:

@@ -716,3 +716,30 @@ def test_step_says_what_a_request_sees():
     assert int(st.status) == 1 and st.seen.tolist() == [0, 4, 16]
     st = ops.kv_step(_i32([5, 9, 2]), _i32([4, 4, 5]), _i32([0, 1, 2, 3]), _i32([3]), _i32([[0, -1], [1, -1], [2, -1]]), 16, 10)
     assert int(st.status) == 8 and st.seen.tolist() == [9, 13, 0]
+
+
+def test_out_and_queries_of_one_storage():
+    """Two ranges of one arena are fine; ranges that overlap are refused, by a single element too."""
+    from b200q import ops
+
+    q, kc, vc, k2, v2, table, ln, _ = _attention_case([40, 21], [1, 1], 1, 4, 64, 16, torch.bfloat16)
+    want = ops.nvfp4_kv_attention(q, kc, vc, k2, v2, table, ln)
+    n = q.numel()
+    arena = torch.zeros(3 * n, dtype=q.dtype, device=DEV)
+    arena[n:2 * n] = q.flatten()
+    mine = arena[n:2 * n].view_as(q)
+    for at in (0, 2 * n):
+        out = arena[at:at + n].view_as(q)
+        assert ops.nvfp4_kv_attention(mine, kc, vc, k2, v2, table, ln, out=out) is out and torch.equal(out, want)
+    assert torch.equal(mine, q)
+    for at in (8, n - 8, n, n + 8, 2 * n - 8):
+        with pytest.raises(ValueError, match="share"):
+            ops.nvfp4_kv_attention(mine, kc, vc, k2, v2, table, ln, out=arena[at:at + n].view_as(q))
+    # strided queries reach as far as their last element
+    wide = torch.zeros(2, 3, 4, 64, dtype=q.dtype, device=DEV)
+    wide[:, 0] = q
+    flat = wide.view(-1)
+    with pytest.raises(ValueError, match="share"):
+        ops.nvfp4_kv_attention(wide[:, 0], kc, vc, k2, v2, table, ln, out=flat[n // 2:n // 2 + n].view_as(q))
+    out = flat[2 * n:3 * n].view_as(q)                       # behind the last query
+    assert torch.equal(ops.nvfp4_kv_attention(wide[:, 0], kc, vc, k2, v2, table, ln, out=out), want)
