@@ -54,7 +54,8 @@ def _only_weight_quantizer_enabled(module) -> bool:
 def enable_real_quant_gemm(model: nn.Module, weight_only: bool = False) -> None:
     """Mark every module whose input and weight quantisers are both enabled to use a registered
     real-quant GEMM.  ``weight_only`` marks those too whose weight quantiser alone is enabled: with a packed
-    4-bit weight and few rows they then read the packed weight instead of dequantising it first."""
+    4-bit weight and few rows they then read the packed weight instead of dequantising it first.  Without it, layers that
+    an earlier call marked in that way lose the mark: the last call says which layers are marked."""
     for module in model.modules():
         if _both_quantizers_enabled(module):
             _set_weight_only(module, False)
@@ -62,6 +63,9 @@ def enable_real_quant_gemm(model: nn.Module, weight_only: bool = False) -> None:
         elif weight_only and _only_weight_quantizer_enabled(module):
             _set_weight_only(module, True)
             module._use_real_quant_gemm = True
+        elif getattr(module, "_weight_only_gemm", False):
+            _set_weight_only(module, False)
+            module._use_real_quant_gemm = False
 
 
 def _set_weight_only(module: nn.Module, value: bool) -> None:

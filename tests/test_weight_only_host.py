@@ -62,3 +62,17 @@ def test_switch_marks_weight_only_layers_when_asked():
     assert mtq.backends.is_real_quant_gemm_enabled(model)
     mtq.backends.disable_real_quant_gemm(model)
     assert not mtq.backends.is_real_quant_gemm_enabled(model)
+
+
+def test_the_last_call_says_which_layers_are_marked():
+    import b200q as mtq
+
+    model = nn.Sequential(nn.Linear(128, 16))
+    mtq.replace_quant_module(model)
+    mtq.set_quantizer_by_cfg(model, mtq.INT4_BLOCKWISE_WEIGHT_ONLY_CFG["quant_cfg"])
+    mtq.backends.enable_real_quant_gemm(model, weight_only=True)
+    assert mtq.backends.is_real_quant_gemm_enabled(model)
+    mtq.backends.enable_real_quant_gemm(model)               # weight-only layers are not asked for any more
+    assert not mtq.backends.is_real_quant_gemm_enabled(model)
+    mtq.backends.enable_real_quant_gemm(model, weight_only=True)
+    assert mtq.backends.is_real_quant_gemm_enabled(model)
