@@ -31,6 +31,8 @@ def _scale2(quantizer, what: str) -> torch.Tensor:
     if getattr(quantizer, "_rotate", False):
         raise NotImplementedError(f"b200q: the {what} quantiser rotates its input; rotate queries and keys before the cache "
                                   "and use a quantiser without rotation")
+    if getattr(quantizer, "pre_quant_scale", None) is not None:
+        raise NotImplementedError(f"b200q: the {what} quantiser has a pre-quant scale, which the cache does not apply")
     s = get_scaling_factor(quantizer)
     if s is None or s.numel() != 1:
         raise ValueError(f"b200q: the {what} quantiser has no calibrated per-tensor amax")

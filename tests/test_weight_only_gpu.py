@@ -444,3 +444,14 @@ def test_a_first_call_that_is_not_covered_is_not_remembered(name):
         assert torch.equal(model(x), want) and len(calls) == 2
     finally:
         ops._w4_linear = real
+
+
+def test_cache_refuses_quantisers_with_a_pre_quant_scale():
+    """A scale that the quantiser puts on its input first would be missing from the cache's keys."""
+    import b200q as mtq
+
+    good, scaled = _quantizer(4.0), _quantizer(4.0)
+    scaled.pre_quant_scale = torch.full((64,), 0.5, device=DEV)
+    for pair in ((scaled, good), (good, scaled)):
+        with pytest.raises(NotImplementedError, match="pre-quant"):
+            mtq.NVFP4KVCache.from_quantizers([pair], num_pages=4, kv_heads=1, head_dim=64, max_requests=1)
