@@ -455,3 +455,63 @@ def test_cache_refuses_quantisers_with_a_pre_quant_scale():
     for pair in ((scaled, good), (good, scaled)):
         with pytest.raises(NotImplementedError, match="pre-quant"):
             mtq.NVFP4KVCache.from_quantizers([pair], num_pages=4, kv_heads=1, head_dim=64, max_requests=1)
+
+
+def test_cache_of_a_model_calibrated_by_quantize():
+    """``quantize`` with NVFP4_KV_CFG on registered attention modules, a cache from their calibrated quantisers, and each
+    layer's attention against the module's fake-quantised keys and values in 64 bits; a later prompt exceeds the calibrated
+    range.  Counted: the result's half step, P in fp16 (2^-11 of each weight, 2^-25 below its normal range), the scores in
+    fp32 (dim + 8 operations of 2^-23 on the sum of magnitudes, twice in a weight's ratio to the sum) and the fake-quantised
+    values' own fp32 (2^-24, in the scores twice and in the result)."""
+    import b200q as mtq
+
+    heads, group, dim = 2, 3, 64
+
+    class Attention(nn.Module):
+        def forward(self, q, k, v):
+            n = k.shape[0]
+            z = torch.einsum("ihgd,nhd->hgin", q.view(-1, heads, group, dim), k) * dim ** -0.5
+            z = z.masked_fill(torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1), float("-inf"))
+            return torch.einsum("hgin,nhd->ihgd", torch.softmax(z, -1), v).reshape(n, heads * group, dim)
+
+    class QuantAttention(Attention):
+        def _setup(self):
+            self.q_bmm_quantizer, self.k_bmm_quantizer, self.v_bmm_quantizer = (mtq.nn.TensorQuantizer() for _ in range(3))
+
+        def forward(self, q, k, v):
+            return super().forward(self.q_bmm_quantizer(q), self.k_bmm_quantizer(k), self.v_bmm_quantizer(v))
+
+    mtq.register(original_cls=Attention, quantized_cls=QuantAttention)
+    try:
+        model = nn.ModuleList([Attention(), Attention()]).cuda()
+        g = torch.Generator(device=DEV).manual_seed(7)
+
+        def data(n, size):
+            q, k, v = (torch.randn(n, h, dim, generator=g, device=DEV) for h in (heads * group, heads, heads))
+            return [t.bfloat16().float() for t in (q, k * size, v * size)]
+
+        calibration = [data(50, 1.0 + i) for i in range(2)]
+        mtq.quantize(model, copy.deepcopy(mtq.NVFP4_KV_CFG), lambda m: [m[i](*calibration[i]) for i in range(2)])
+        cache = mtq.NVFP4KVCache.from_quantizers([(m.k_bmm_quantizer, m.v_bmm_quantizer) for m in model], num_pages=20,
+                                                 kv_heads=heads, head_dim=dim, max_requests=1, page_size=16)
+        for i, m in enumerate(model):
+            for name, at in (("k", 1), ("v", 2)):
+                amax = calibration[i][at].abs().max()
+                assert abs(float(cache.layers[i][1 + at] / amax * 2688) - 1) < 2.0 ** -22
+        step = cache.step(_int32([90]), 90)
+        cache.check()
+        for i, m in enumerate(model):
+            q, k, v = data(90, (1.0 + i) * 1.5)
+            cache.append(i, k.bfloat16(), v.bfloat16(), step)
+            out = cache.attend(i, q.bfloat16(), step).double()
+            K, V = m.k_bmm_quantizer(k), m.v_bmm_quantizer(v)
+            assert torch.isfinite(K).all() and torch.isfinite(V).all() and float(k.abs().max()) > float(calibration[i][1].abs().max())
+            K, V, Q = K.double(), V.double(), q.double().view(90, heads, group, dim)
+            want = Attention.forward(m, q.double(), K, V)
+            p_abs = Attention.forward(m, q.double(), K, V.abs())
+            big = torch.einsum("ihgd,nhd->hgin", Q.abs(), K.abs()).max() * dim ** -0.5
+            rel = 2.0 ** -11 + 2 * (dim + 12) * 2.0 ** -23 * float(big) + 2.0 ** -20
+            tol = (2.0 ** -8 * want.abs() + rel * p_abs + 90 * 2.0 ** -25 * V.abs().max()) * 1.01
+            assert float(((out - want).abs() - tol).max()) <= 0
+    finally:
+        mtq.unregister(Attention)
