@@ -17,11 +17,27 @@ from .gemm_registry import gemm_registry
 
 __all__ = ["WeightOnlyLinear", "weight_only_gemm", "WEIGHT_ONLY_MAX_ROWS"]
 
-# Rows up to which the packed weight is used; more go through the dequantised weight and a library GEMM.  Measured on
-# 4096 x 4096, 8192 x 8192, 8192 x 28672 and 28672 x 8192 weights (us, packed against dequantised): INT4 at 128 rows
-# 46 / 52, 111 / 226, 272 / 783, 307 / 796 (at 256 rows 92 / 53 on the smallest); NVFP4 at 32 rows 11 / 14, 25 / 53,
-# 60 / 182, 68 / 187 (at 64 rows 21 / 14 on the smallest).
-WEIGHT_ONLY_MAX_ROWS = {INT4QTensor: 128, NVFP4QTensor: 32}
+# Rows up to which any layer uses the packed weight (one launch); more go through the dequantised weight and a library
+# GEMM.  Measured on the device (us, packed against dequantised): at 32 rows INT4 6.6 / 8.3 on 1024 x 1024, 7.5 / 17 on
+# 2048 x 2048, 12.7 / 48 on 4096 x 4096, NVFP4 5.9 / 5.3, 6.9 / 7.3 and 11.6 / 13.5; smaller layers lose up to 3 us from 17
+# rows on, and gain 14 us of host time where calls are not captured.
+WEIGHT_ONLY_MAX_ROWS = {INT4QTensor: 32, NVFP4QTensor: 32}
+
+# INT4 dequantises more slowly, so that large layers gain from several launches too.  A launch costs about 6 us and 0.4 us a
+# million weights, the other path 5 us and 2.7 us a million; and a further launch 10 us of host time, which the last
+# two sizes need to hide: 64 rows 14.6 / 17 us on 2048 x 2048 (12.8 / 8.1 on 1024 x 1024), 128 rows 61 / 72 us on 5120 x 5120
+# (50 / 48 on 4096 x 4096), 272 / 783 on 8192 x 28672; 256 rows 92 / 53 on 4096 x 4096.
+_INT4_MAX_ROWS = 128
+_INT4_WEIGHTS_PER_LAUNCH_PAIR = 1 << 21
+
+
+def _takes_packed(kind, rows: int, n: int, k: int) -> bool:
+    """Whether ``rows`` rows go to the packed [n, k] weight: in one launch, or in several where the weight is large."""
+    if rows <= WEIGHT_ONLY_MAX_ROWS[kind]:
+        return True
+    launches = -(-rows // ops._w4_max_rows(k))
+    return (kind is INT4QTensor and rows <= _INT4_MAX_ROWS
+            and launches * (launches - 1) * _INT4_WEIGHTS_PER_LAUNCH_PAIR <= n * k)
 
 
 def weight_only_gemm(quant_module, input_tensor, bias=None):
@@ -99,7 +115,8 @@ class WeightOnlyLinear(Function):
 
 def _weight_only_linear(quant_module, input, weight, bias=None):
     x = quant_module.input_quantizer(input)               # a disabled quantiser still applies its AWQ pre-quant scale
-    if not _covered(quant_module, x) or x.numel() // x.shape[-1] > WEIGHT_ONLY_MAX_ROWS[weight.metadata["qtensor_class"]]:
+    if not _covered(quant_module, x) or not _takes_packed(weight.metadata["qtensor_class"], x.numel() // x.shape[-1],
+                                                          *weight.metadata["shape"]):
         return F.linear(x, quant_module._quantized_weight(), bias)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return WeightOnlyLinear.apply(quant_module, x, weight, bias)

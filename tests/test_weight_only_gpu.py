@@ -515,3 +515,38 @@ def test_cache_of_a_model_calibrated_by_quantize():
             assert float(((out - want).abs() - tol).max()) <= 0
     finally:
         mtq.unregister(Attention)
+
+
+@pytest.mark.parametrize("name,n,k,packed,dequantised", [
+    ("INT4_BLOCKWISE_WEIGHT_ONLY_CFG", 512, 512, [1, 32], [33, 64, 128]),
+    ("INT4_BLOCKWISE_WEIGHT_ONLY_CFG", 2048, 2048, [32, 33, 64], [65, 128]),
+    ("INT4_BLOCKWISE_WEIGHT_ONLY_CFG", 5120, 5120, [64, 65, 128], [129]),
+    ("NVFP4_MLP_WEIGHT_ONLY_CFG", 2048, 2048, [1, 32], [33])])
+def test_rows_that_take_several_launches_need_a_large_layer(name, n, k, packed, dequantised):
+    """Several launches of the packed product only where the weight is large enough to pay for them."""
+    import b200q as mtq
+    from b200q import ops
+
+    class Layer(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.mlp = nn.Linear(k, n, bias=False)
+
+    model = Layer().bfloat16().cuda()
+    mtq.quantize(model, copy.deepcopy(getattr(mtq, name)), lambda m: None)
+    mtq.compress(model, {"weight_only_gemm": True})
+    calls, real = [], ops._w4_linear
+    try:
+        ops._w4_linear = lambda *a, **kw: (calls.append(a[0]), real(*a, **kw))[1]
+        for rows in packed + dequantised:
+            x = torch.randn(rows, k, device=DEV, dtype=torch.bfloat16)
+            calls.clear()
+            with torch.no_grad():
+                got = model.mlp(x)
+                assert len(calls) == (rows in packed), rows
+                want = F.linear(x, model.mlp.weight_quantizer.dequantize(model.mlp.weight))
+            size = x.float().abs() @ model.mlp.weight_quantizer.dequantize(model.mlp.weight).float().abs().t()
+            # weights rounded to bf16 on one side, outputs on both
+            assert float(((got.float() - want.float()).abs() - 3 * 2.0 ** -8 * size).max()) <= 0
+    finally:
+        ops._w4_linear = real
