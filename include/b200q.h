@@ -39,6 +39,9 @@ const char* b200q_strerror(int status);
 int b200q_version(void);
 /* number of SMs of the current device (grid sizing is a multiple of it) */
 int b200q_sm_count(void);
+/* *word = address of a device word of the current device, zero when the library is loaded, for the status_io of products
+ * that run there (it may be asked for while a stream is capturing). */
+int b200q_gemm_status_word(uint32_t** word);
 
 /* ---------------------------------------------------------------- amax reductions --------- */
 

@@ -33,6 +33,7 @@ SIGNATURES = {
     "b200q_strerror": [_i],
     "b200q_version": [],
     "b200q_sm_count": [],
+    "b200q_gemm_status_word": [_p],
     "b200q_amax_tensor": [_p, _i64, _i, _p, _p],
     "b200q_amax_axis": [_p, _i64, _i64, _i64, _i, _p, _p],
     "b200q_amax_blocks": [_p, _i64, _i, _i, _p, _p],

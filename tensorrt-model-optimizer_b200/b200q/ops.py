@@ -803,7 +803,23 @@ def qgemm_status(device) -> torch.Tensor:
         device = torch.device("cuda", torch.cuda.current_device())
     st = _QGEMM_STATUS.get(device)
     if st is None:
-        st = _QGEMM_STATUS[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        st = _QGEMM_STATUS[device] = _status_word(device)
+    return st
+
+
+def _status_word(device) -> torch.Tensor:
+    """The library's own word on ``device`` as a tensor.  An allocated one would be zeroed by every replay of a graph
+    whose capture made the first product, and lose the error bits collected so far."""
+    word = ctypes.c_void_p()
+    with torch.cuda.device(device):
+        call("b200q_gemm_status_word", ctypes.addressof(word))
+
+    class Word:
+        __cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (word.value, False), "version": 3, "strides": None}
+
+    st = torch.as_tensor(Word(), device=device)
+    if st.data_ptr() != word.value:
+        raise RuntimeError("b200q: the status word could not be shared with torch")
     return st
 
 

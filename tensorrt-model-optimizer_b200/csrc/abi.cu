@@ -20,3 +20,17 @@ extern "C" const char* b200q_strerror(int status) {
 extern "C" int b200q_version(void) { return 100; }
 
 extern "C" int b200q_sm_count(void) { return b200q::sm_count_cached(); }
+
+// The error word of a device's products.  A variable of the module, zero when that is loaded: it needs no allocation and no
+// fill, which a stream under capture would record and repeat with every replay.
+namespace b200q {
+__device__ uint32_t g_gemm_status;
+}
+
+extern "C" int b200q_gemm_status_word(uint32_t** word) {
+  B200Q_REQUIRE_PTR(word);
+  void* at = nullptr;
+  if (cudaGetSymbolAddress(&at, b200q::g_gemm_status) != cudaSuccess) return B200Q_ERR_CUDA;
+  *word = static_cast<uint32_t*>(at);
+  return B200Q_OK;
+}

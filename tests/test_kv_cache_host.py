@@ -73,3 +73,21 @@ def test_status_codes():
     for kw in (dict(q=p + 8), dict(qs=65), dict(qh=4), dict(kc=p + 8), dict(out=p + 4), dict(ws=p + 8)):
         assert attention(**kw) == ALIGN, kw
     assert lib.b200q_nvfp4_kv_attention_workspace(1, 1, 1, 1, 96) == SHAPE
+
+
+def test_status_codes_of_the_step_that_says_what_is_seen():
+    from b200q import _cabi
+
+    buf = ctypes.create_string_buffer(512)
+    p = (ctypes.addressof(buf) + 31) & ~31
+
+    def step(**kw):
+        a = dict(lens=p, new=p, free=p, nfree=1, taken=p, table=p, stride=1, width=1, requests=1, page=16, tokens=1, slots=p,
+                 positions=p, cu=p, lens_out=p, taken_out=p, status=p, seen=p)
+        a.update(kw)
+        return _cabi.lib.b200q_kv_step_seen(*a.values(), None)
+
+    for name in ("lens", "new", "free", "taken", "table", "slots", "positions", "cu", "lens_out", "taken_out", "status"):
+        assert step(**{name: None}) == -1, name
+    assert step(requests=0) == -4 and step(stride=0) == -4 and step(requests=8193) == -7
+    assert step(requests=8193, seen=None) == -7

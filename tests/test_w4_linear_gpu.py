@@ -309,3 +309,38 @@ def test_ctas_that_walk_over_several_tiles(m, n, k, fmt, block, dtype):
         top = torch.maximum(ref.abs(), got.abs()).clamp(min=info.tiny)
         half = torch.exp2(torch.floor(torch.log2(top))) * info.eps / 2
         assert float(((got - ref).abs() - half - size * adds * 2.0 ** -24 - own).max()) <= 0
+
+
+def test_replays_keep_the_error_word():
+    """A first product under capture: replays must not clear the error bits that were collected before them.  In a process
+    of its own, since the word is made by a process's first product."""
+    import subprocess
+    import sys
+
+    code = """
+import sys
+sys.path[:0] = %r
+import torch
+from b200q import ops
+packed, scales = ops.int4_quantize(torch.randn(64 * 512, device="cuda").bfloat16(), 128)
+packed = packed.view(64, 256)
+x = torch.randn(3, 512, device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = ops.int4_linear(x, packed, scales, 128)
+ops.check_qgemm_status("cuda")                          # clean before the first replay
+graph.replay()
+ops.check_qgemm_status("cuda")
+assert torch.equal(out, ops.int4_linear(x, packed, scales, 128))
+ops.qgemm_status("cuda").fill_(4)                       # as a wait that ran out would leave it
+graph.replay()
+try:
+    ops.check_qgemm_status("cuda")
+except RuntimeError:
+    ops.check_qgemm_status("cuda")                      # told once
+else:
+    raise AssertionError("the error bits are lost")
+""" % sys.path
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -76,3 +76,9 @@ def test_the_last_call_says_which_layers_are_marked():
     assert not mtq.backends.is_real_quant_gemm_enabled(model)
     mtq.backends.enable_real_quant_gemm(model, weight_only=True)
     assert mtq.backends.is_real_quant_gemm_enabled(model)
+
+
+def test_status_word_needs_a_place_for_its_address():
+    from b200q import _cabi
+
+    assert _cabi.lib.b200q_gemm_status_word(None) == -1
