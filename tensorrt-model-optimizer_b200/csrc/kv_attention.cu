@@ -25,12 +25,13 @@
 // one contiguous run of the row: D/4 dimensions of one token for K, D/8 dimensions of four tokens for V, whose nibbles
 // are interleaved so that one conversion gives the same dimension of two neighbouring tokens.
 //
-// What bounds it.  The fetches alone run at 6.3 TB/s (0.95 of the copy rate); with the products 4.2 to 4.8 TB/s: 295
+// What bounds it.  The fetches alone run at 6.3 TB/s (0.95 of the copy rate); with the products 4.2 to 4.8 TB/s: 297
 // instructions per 16 tokens of a head of 128, 64 of them conversions and 64 multiplies that issue every other cycle, at
 // 0.6 instructions a cycle and scheduler with three warps each.  Measured (device time): 64 requests of 17 to 8192
-// tokens, 8 kv heads, group 4, D 128: 69 us for 287 MB; 8 x 65536 tokens, group 8: 127 us for 604 MB; 16 requests with up
-// to 8 queries, D 256: 29 us for 39 MB.  Four blocks of 128 registers an SM measured 74 / 132 us, blocks of 5, 7, 14 or 16
-// warps 81 / 147, 85 / 149, 88 / 142 and 83 / 135 us, bulk copies instead of cp.async 80 / 145 (four blocks).
+// tokens, 8 kv heads, group 4, D 128: 69 us for 287 MB (72 with cu_q); 8 x 65536 tokens, group 8: 125 to 135 us for 604 MB
+// (165 to 172 with cu_q); 16 requests with up to 8 queries, D 256: 29 us for 39 MB.  Four blocks of 128 registers an SM
+// measured 74 / 132 us, blocks of 5, 7, 14 or 16 warps 81 / 147, 85 / 149, 88 / 142 and 83 / 135 us, bulk copies instead of
+// cp.async 80 / 145 (four blocks).
 #include "umma.cuh"
 
 namespace b200q {
